@@ -163,6 +163,67 @@ int i8moe_moe_unpermute(const void* permuted_hidden, int dtype, const float* top
                         int64_t n_token, int64_t topk, int64_t n_hidden, void* out,
                         i8moe_stream_t stream);
 
+/* Rows to the experts and back in training (no reference counterpart).  The
+ * maps and offsets are those of i8moe_moe_permute_metadata; sorted rows past
+ * expert_first_token_offset[n_local_expert] (NULL: none) belong to no local
+ * expert.  Rows and gradients of a dtype (I8MOE_BF16 / FP16 / FP32), row
+ * bytes a multiple of 16, pointers 16-byte aligned; sums fp32 in top-k order,
+ * rounded once; no atomics, so results repeat bit for bit.
+ *
+ * moe_scatter_rows: the row copy of i8moe_moe_permute from given maps,
+ *   permuted_input[inv[t, j]] = input[t], and zeros in the rows past the
+ *   local experts' (i8moe_moe_permute leaves those as they were). */
+int i8moe_moe_scatter_rows(const void* input, int dtype, const int32_t* inv_permuted_idx,
+                           const int64_t* expert_first_token_offset, int64_t n_local_expert,
+                           int64_t n_token, int64_t topk, int64_t n_hidden, void* permuted_input,
+                           i8moe_stream_t stream);
+/* The row copy's gradient: input_grad[t] = sum_j permuted_grad[inv[t, j]]
+ * over the rows of local experts. */
+int i8moe_moe_permute_backward(const void* permuted_grad, int dtype,
+                               const int32_t* inv_permuted_idx,
+                               const int64_t* expert_first_token_offset, int64_t n_local_expert,
+                               int64_t n_token, int64_t topk, int64_t n_hidden, void* input_grad,
+                               i8moe_stream_t stream);
+/* i8moe_moe_unpermute's gradients: permuted_grad[inv[t, j]] = topk_weights[t, j]
+ * * out_grad[t] and weights_grad[t, j] = <out_grad[t], permuted_hidden[inv[t, j]]>
+ * (fp32); both 0 for rows of no local expert, which are not read. */
+int i8moe_moe_unpermute_backward(const void* out_grad, const void* permuted_hidden, int dtype,
+                                 const float* topk_weights, const int32_t* inv_permuted_idx,
+                                 const int64_t* expert_first_token_offset, int64_t n_local_expert,
+                                 int64_t n_token, int64_t topk, int64_t n_hidden,
+                                 void* permuted_grad, float* weights_grad, i8moe_stream_t stream);
+
+/* ---------------------------------------------------------------- norm */
+
+/* No reference counterpart: the residual's addition and the RMS norm in front
+ * of the layer.  Per row of n_hidden elements (row strides in elements; the
+ * outputs are dense):
+ *   h = x + residual          (without residual: h = x)
+ *   y = h / sqrt(mean(h^2) + eps) * weight
+ *   q_scale = max(max|y|, 1e-10) / 127,  q = rint(y / q_scale)
+ * in fp32 from the unrounded h and y; residual_out (with residual only), y
+ * and q are rounded once.  y, rstd (fp32 [n_rows], for the backward pass) and
+ * q / q_scale may be NULL, not both y and q.  A row whose norm is not finite
+ * gets q_scale NaN and q 0.  weight has the rows' dtype or I8MOE_FP32. */
+int i8moe_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                   int dtype, const void* weight, int weight_dtype, int64_t n_rows,
+                   int64_t n_hidden, float eps, void* residual_out, void* y, float* rstd,
+                   int8_t* q, float* q_scale, i8moe_stream_t stream);
+/* Bytes of scratch that i8moe_rms_norm_backward needs when it is given
+ * dweight. */
+size_t i8moe_rms_norm_backward_workspace_size(int64_t n_rows, int64_t n_hidden);
+/* Gradients: with n = h * rstd and a = dy * weight,
+ *   dx = rstd * (a - n * mean(a * n)) + residual_grad   (x's and residual's)
+ *   dweight = sum over rows of dy * n
+ * h is residual_out (x without a residual), rstd as i8moe_rms_norm wrote it,
+ * residual_grad the gradient of residual_out or NULL; dweight may be NULL.
+ * Sums are fp32 in a fixed order. */
+int i8moe_rms_norm_backward(const void* dy, int64_t dy_stride, const void* residual_grad,
+                            int64_t residual_grad_stride, const void* h, int64_t h_stride,
+                            int dtype, const void* weight, int weight_dtype, const float* rstd,
+                            int64_t n_rows, int64_t n_hidden, void* dx, void* dweight,
+                            void* workspace, size_t workspace_bytes, i8moe_stream_t stream);
+
 /* ---------------------------------------------------------- activation */
 
 /* Replaces silu_and_mul (csrc/activation_kernels.cu:260-265):
@@ -289,6 +350,30 @@ int i8moe_int8_grouped_mm(const int8_t* a, const int8_t* b, void* out, int out_d
                           const int32_t* expert_offsets, const int32_t* problem_sizes,
                           int64_t n_expert, int64_t sum_m, int64_t n, int64_t k,
                           i8moe_stream_t stream);
+
+/* 4-bit weights for decoding (no reference counterpart).  packed [E, N, K / 2]
+ * holds column k of a row in byte k / 2, low half for even k, as q + 8 with q
+ * in [-8, 7]; scale [E, N, ceil(K / group_size)] of scale_dtype.  Per group:
+ * scale = max|w| / 7 rounded to its type, q = clamp(rint(w / scale), -8, 7)
+ * (ties to even) by the rounded scale; a group of zeros has scale 0.
+ * group_size 32, 64 or 128; K a multiple of 32. */
+int i8moe_quantize_weights_int4(const void* w, int dtype, int64_t n_expert, int64_t n, int64_t k,
+                                int64_t group_size, uint8_t* packed, void* scale, int scale_dtype,
+                                i8moe_stream_t stream);
+/* Products of each expert's rows with its 4-bit weights, for few rows per
+ * expert:
+ *   y[r, n] = sum_k x[src(r), k] * scale[e, n, k / group_size] * q[e, n, k]
+ * for expert_offsets[e] <= r < expert_offsets[e + 1] (int32 [E + 1]), src(r) = r,
+ * or permuted_idx[r] / topk when that is non-NULL.  out [n_rows, n] = y; with
+ * silu != 0 out [n_rows, n / 2] = silu(y[:, :n/2]) * y[:, n/2:].  Sums are
+ * fp32, rounded once at the end.  Rows outside every expert keep what they
+ * held.  x bf16 / fp16 with rows x_stride elements apart (16-byte aligned),
+ * out of x's dtype, scale of x's dtype or fp32. */
+int i8moe_int4_grouped_mv(const void* x, int64_t x_stride, int64_t x_rows, int dtype,
+                          const int32_t* permuted_idx, int64_t topk, const uint8_t* w_packed,
+                          const void* w_scale, int scale_dtype, int64_t group_size,
+                          const int32_t* expert_offsets, int64_t n_expert, int64_t n_rows,
+                          int64_t n, int64_t k, int silu, void* out, i8moe_stream_t stream);
 
 /* Grouped-GEMM variant (no reference counterpart; results are identical
  * either way).  mode 1: every hybrid grouped GEMM above runs on CTA pairs --

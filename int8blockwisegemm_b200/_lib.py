@@ -13,6 +13,8 @@ import os
 from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p
 from pathlib import Path
 
+import torch
+
 _DEFAULT_LIB_PATH = str(Path(__file__).resolve().parent / "libi8moe.so")
 LIB_PATH = os.environ.get("INT8_HYBRID_MOE_LIB", _DEFAULT_LIB_PATH)
 
@@ -50,6 +52,13 @@ PROTOTYPES = {
     "i8moe_moe_permute": (I32, [P, I32, I64, P, P, P, I64, I64, I64, I64, P, P, P, P, P, c_size_t,
                                 P]),
     "i8moe_moe_unpermute": (I32, [P, I32, P, P, P, I64, I64, I64, I64, P, P]),
+    "i8moe_moe_scatter_rows": (I32, [P, I32, P, P, I64, I64, I64, I64, P, P]),
+    "i8moe_moe_permute_backward": (I32, [P, I32, P, P, I64, I64, I64, I64, P, P]),
+    "i8moe_moe_unpermute_backward": (I32, [P, P, I32, P, P, P, I64, I64, I64, I64, P, P, P]),
+    "i8moe_rms_norm": (I32, [P, I64, P, I64, I32, P, I32, I64, I64, c_float, P, P, P, P, P, P]),
+    "i8moe_rms_norm_backward_workspace_size": (c_size_t, [I64, I64]),
+    "i8moe_rms_norm_backward": (I32, [P, I64, P, I64, P, I64, I32, P, I32, P, I64, I64, P, P, P,
+                                      c_size_t, P]),
     "i8moe_silu_and_mul": (I32, [P, P, I32, I64, I64, P]),
     "i8moe_scale_offsets": (I32, [P, I64, I64, P, P]),
     "i8moe_quant_grouped": (I32, [P, I32, I64, I64, P, I64, I64, I64, I64, I64, P, P, P, P, I32,
@@ -65,6 +74,9 @@ PROTOTYPES = {
                                                    I64, I64, I64, I64, I64, I64, I64, I64, P, P,
                                                    P, P]),
     "i8moe_int8_grouped_mm": (I32, [P, P, P, I32, c_float, P, P, P, P, I64, I64, I64, I64, P]),
+    "i8moe_quantize_weights_int4": (I32, [P, I32, I64, I64, I64, I64, P, P, I32, P]),
+    "i8moe_int4_grouped_mv": (I32, [P, I64, I64, I32, P, I64, P, P, I32, I64, P, I64, I64, I64,
+                                    I64, I32, P, P]),
     "i8moe_gemm_set_cta_pairs": (I32, [I32]),
     "i8moe_int8_mma_peak": (I32, [I64, I32, P, P]),
 }
@@ -102,6 +114,19 @@ def check(rc: int, what: str = "") -> None:
 
 def call(name: str, *args) -> None:
     check(getattr(LIB, name)(*args), name)
+
+
+def launch(name: str, device, *args) -> None:
+    """Call an entry point on the current stream of ``device``, which is made
+    the current device for the call when it is not."""
+    fn = getattr(LIB, name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != 0:
+        check(rc, name)
 
 
 def set_cta_pairs(mode: int) -> int:

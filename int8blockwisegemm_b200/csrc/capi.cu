@@ -50,6 +50,8 @@ int read_quant_error(uint32_t* w, int clear);
 int read_gemm_error(uint32_t* w, int clear);
 int read_ep_error(uint32_t* w, int clear);
 int read_peak_error(uint32_t* w, int clear);
+int read_route_grad_error(uint32_t* w, int clear);
+int read_int4_error(uint32_t* w, int clear);
 
 }  // namespace i8moe
 
@@ -71,8 +73,11 @@ int i8moe_device_error(int device, uint32_t* word, int clear) {
   uint32_t d = 0, e = 0;
   if (rc == I8MOE_OK) rc = i8moe::read_ep_error(&d, clear);
   if (rc == I8MOE_OK) rc = i8moe::read_peak_error(&e, clear);
+  uint32_t f = 0, g = 0;
+  if (rc == I8MOE_OK) rc = i8moe::read_route_grad_error(&f, clear);
+  if (rc == I8MOE_OK) rc = i8moe::read_int4_error(&g, clear);
   cudaSetDevice(prev);
-  if (word) *word = a | b | c | d | e;
+  if (word) *word = a | b | c | d | e | f | g;
   return rc;
 }
 

@@ -1,0 +1,130 @@
+"""Expert layers with 4-bit weights and group scales for decoding (no
+reference counterpart): the weights' quantisation, the products of each
+expert's few rows, and the layer's forward.
+
+Weights are kept as ``packed`` uint8 [E, N, K/2], column k in byte k // 2 (low
+half for even k) as q + 8 with q in [-8, 7], and ``scale`` [E, N,
+ceil(K / group_size)]; a weight is scale * q.  Activations are bf16 or fp16.
+The kernels read the weights of the experts that have rows once per eight
+rows, so they are for few rows per expert; with many, the INT8 grouped GEMMs
+are the faster way.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from ._lib import BF16, FP16, FP32, launch
+from .permute import moe_route_for_gemm, moe_unpermute
+
+_DT = {torch.bfloat16: BF16, torch.float16: FP16, torch.float32: FP32}
+
+
+def _check(cond: bool, msg: str) -> None:
+    if not cond:
+        raise RuntimeError(msg)
+
+
+def quantize_weights_int4(w: torch.Tensor, group_size: int = 128, scale_dtype=None):
+    """(packed, scale) of w [E, N, K] (bf16, fp16 or fp32): per group
+    scale = max|w| / 7 rounded to ``scale_dtype`` (w's type when omitted) and
+    q = clamp(rint(w / scale), -8, 7).  K must be a multiple of 32,
+    group_size 32, 64 or 128; the last group of a row may be shorter."""
+    scale_dtype = w.dtype if scale_dtype is None else scale_dtype
+    _check(w.is_cuda and w.dim() == 3, "quantize_weights_int4: w must be a CUDA tensor [E, N, K]")
+    _check(w.dtype in _DT and scale_dtype in _DT, "quantize_weights_int4: unsupported dtype")
+    _check(group_size in (32, 64, 128),
+           "quantize_weights_int4: group_size must be 32, 64 or 128")
+    E, N, K = w.shape
+    _check(K % 32 == 0, "quantize_weights_int4: K must be divisible by 32")
+    w = w.contiguous()
+    packed = torch.empty((E, N, K // 2), dtype=torch.uint8, device=w.device)
+    scale = torch.empty((E, N, -(-K // group_size)), dtype=scale_dtype, device=w.device)
+    launch("i8moe_quantize_weights_int4", w.device, w.data_ptr(), _DT[w.dtype], E, N, K,
+           group_size, packed.data_ptr(), scale.data_ptr(), _DT[scale_dtype])
+    return packed, scale
+
+
+def int4_grouped_mv(x, w_packed, w_scale, expert_offsets, group_size: int = 128,
+                    permuted_idx=None, topk: int = 1, silu: bool = False, out=None):
+    """Rows r in [expert_offsets[e], expert_offsets[e+1]) times the transposed
+    weights of expert e.
+
+    x [rows, K] holds the sorted rows; with ``permuted_idx`` (int32 [rows])
+    row r is x[permuted_idx[r] // topk] instead.  ``silu``: w_packed holds N/2
+    gate rows and then N/2 up rows, and the result is silu(gate) * up.
+    Returns ``out`` [rows, N] (N/2 with silu) in x's type, allocated when not
+    given; rows outside every expert keep what it held.  Sums are fp32,
+    rounded once."""
+    _check(x.is_cuda and x.dim() == 2, "int4_grouped_mv: x must be a CUDA tensor [rows, K]")
+    _check(x.dtype in (torch.bfloat16, torch.float16),
+           "int4_grouped_mv: x must be bfloat16 or float16")
+    dev = x.device
+    _check(w_packed.dtype == torch.uint8 and w_packed.dim() == 3 and w_packed.is_contiguous()
+           and w_packed.device == dev,
+           "int4_grouped_mv: w_packed must be contiguous uint8 [E, N, K/2] on x's device")
+    E, N, half = w_packed.shape
+    K = 2 * half
+    _check(group_size in (32, 64, 128), "int4_grouped_mv: group_size must be 32, 64 or 128")
+    _check(x.size(1) == K, "int4_grouped_mv: x.shape[1] must be twice w_packed.shape[2]")
+    _check(K >= 32 and K % 32 == 0, "int4_grouped_mv: K must be positive and divisible by 32")
+    _check(w_scale.dtype in (x.dtype, torch.float32),
+           "int4_grouped_mv: w_scale must have x's dtype or float32")
+    _check(w_scale.shape == (E, N, -(-K // group_size)) and w_scale.is_contiguous()
+           and w_scale.device == dev,
+           "int4_grouped_mv: w_scale must be contiguous [E, N, ceil(K / group_size)] on x's device")
+    _check(expert_offsets.dtype == torch.int32 and expert_offsets.shape == (E + 1,)
+           and expert_offsets.is_contiguous() and expert_offsets.device == dev,
+           "int4_grouped_mv: expert_offsets must be contiguous int32 [E + 1] on x's device")
+    _check(not silu or N % 2 == 0, "int4_grouped_mv: N must be even with silu")
+    rows = x.size(0)
+    if permuted_idx is not None:
+        _check(permuted_idx.dtype == torch.int32 and permuted_idx.dim() == 1
+               and permuted_idx.is_contiguous() and permuted_idx.device == dev,
+               "int4_grouped_mv: permuted_idx must be contiguous int32 [rows] on x's device")
+        _check(topk >= 1, "int4_grouped_mv: topk must be positive")
+        rows = permuted_idx.size(0)
+    n_out = N // 2 if silu else N
+    if out is None:
+        out = torch.empty((rows, n_out), dtype=x.dtype, device=dev)
+    else:
+        _check(out.dtype == x.dtype and out.shape == (rows, n_out) and out.is_contiguous()
+               and out.device == dev,
+               "int4_grouped_mv: out must be contiguous [rows, N (N/2 with silu)] of x's dtype "
+               "on x's device")
+    if x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.stride(0) < K or x.data_ptr() % 16 != 0:
+        x = x.contiguous() if x.data_ptr() % 16 == 0 else x.clone(
+            memory_format=torch.contiguous_format)
+    launch("i8moe_int4_grouped_mv", dev, x.data_ptr(), K if x.size(0) < 2 else x.stride(0),
+           x.size(0), _DT[x.dtype], permuted_idx.data_ptr() if permuted_idx is not None else None,
+           topk, w_packed.data_ptr(), w_scale.data_ptr(), _DT[w_scale.dtype], group_size,
+           expert_offsets.data_ptr(), E, rows, N, K, 1 if silu else 0, out.data_ptr())
+    return out
+
+
+def run_int4_moe(output, hidden_states, w1_packed, w1_scale, w2_packed, w2_scale, topk_ids,
+                 topk_weights, global_num_experts: int, expert_map=None,
+                 group_size: int = 128) -> None:
+    """MoE forward of a decoding step with 4-bit weights; writes ``output``
+    [T, K].  w1 [E, 2N, K] (gate rows, then up rows) and w2 [E, K, N] as
+    ``quantize_weights_int4`` packs them, E being the local experts;
+    ``expert_map`` as in the INT8 forward.  Six launches, no host
+    synchronisation; it can be captured into a CUDA graph."""
+    _check(hidden_states.dim() == 2 and w1_packed.dim() == 3 and w2_packed.dim() == 3,
+           "run_int4_moe: hidden_states must be [T, K], the weights [E, rows, columns / 2]")
+    T, K = hidden_states.shape
+    E, two_n, _ = w1_packed.shape
+    _check(2 * w1_packed.size(2) == K and w2_packed.shape == (E, K, two_n // 4) and two_n % 4 == 0,
+           "run_int4_moe: w1 must be [E, 2N, K] and w2 [E, K, N]")
+    _check(topk_ids.dim() == 2 and topk_ids.size(0) == T and topk_weights.shape == topk_ids.shape,
+           "run_int4_moe: topk_ids and topk_weights must have shape [T, topk]")
+    _check(output.shape == hidden_states.shape and output.dtype == hidden_states.dtype
+           and output.is_contiguous() and output.device == hidden_states.device,
+           "run_int4_moe: output must be contiguous [T, K] of hidden_states' dtype and device")
+    topk = topk_ids.size(1)
+    eft, inv, pidx, eo, _, _, _ = moe_route_for_gemm(
+        topk_ids.contiguous(), T, global_num_experts, E, expert_map, two_n, K, K, two_n // 2, 64)
+    act = int4_grouped_mv(hidden_states, w1_packed, w1_scale, eo, group_size, permuted_idx=pidx,
+                          topk=topk, silu=True)
+    mm2 = int4_grouped_mv(act, w2_packed, w2_scale, eo, group_size)
+    moe_unpermute(output, mm2, topk_weights.contiguous(), inv, eft)
