@@ -75,8 +75,8 @@ PROTOTYPES = {
                                                    P, P]),
     "i8moe_int8_grouped_mm": (I32, [P, P, P, I32, c_float, P, P, P, P, I64, I64, I64, I64, P]),
     "i8moe_quantize_weights_int4": (I32, [P, I32, I64, I64, I64, I64, P, P, I32, P]),
-    "i8moe_int4_grouped_mv": (I32, [P, I64, I64, I32, P, I64, P, P, I32, I64, P, I64, I64, I64,
-                                    I64, I32, P, P]),
+    "i8moe_int4_grouped_mv": (I32, [P, I64, I64, I32, P, I64, P, P, I64, P, I64, I64, I64, I64,
+                                    I32, P, P]),
     "i8moe_gemm_set_cta_pairs": (I32, [I32]),
     "i8moe_int8_mma_peak": (I32, [I64, I32, P, P]),
 }

@@ -68,8 +68,7 @@ def int4_grouped_mv(x, w_packed, w_scale, expert_offsets, group_size: int = 128,
     _check(group_size in (32, 64, 128), "int4_grouped_mv: group_size must be 32, 64 or 128")
     _check(x.size(1) == K, "int4_grouped_mv: x.shape[1] must be twice w_packed.shape[2]")
     _check(K >= 32 and K % 32 == 0, "int4_grouped_mv: K must be positive and divisible by 32")
-    _check(w_scale.dtype in (x.dtype, torch.float32),
-           "int4_grouped_mv: w_scale must have x's dtype or float32")
+    _check(w_scale.dtype == x.dtype, "int4_grouped_mv: w_scale must have x's dtype")
     _check(w_scale.shape == (E, N, -(-K // group_size)) and w_scale.is_contiguous()
            and w_scale.device == dev,
            "int4_grouped_mv: w_scale must be contiguous [E, N, ceil(K / group_size)] on x's device")
@@ -97,7 +96,7 @@ def int4_grouped_mv(x, w_packed, w_scale, expert_offsets, group_size: int = 128,
             memory_format=torch.contiguous_format)
     launch("i8moe_int4_grouped_mv", dev, x.data_ptr(), K if x.size(0) < 2 else x.stride(0),
            x.size(0), _DT[x.dtype], permuted_idx.data_ptr() if permuted_idx is not None else None,
-           topk, w_packed.data_ptr(), w_scale.data_ptr(), _DT[w_scale.dtype], group_size,
+           topk, w_packed.data_ptr(), w_scale.data_ptr(), group_size,
            expert_offsets.data_ptr(), E, rows, N, K, 1 if silu else 0, out.data_ptr())
     return out
 

@@ -94,14 +94,13 @@ SHAPES = [  # counts, N, K
 @pytest.mark.parametrize("G", [32, 64, 128])
 @pytest.mark.parametrize("counts,N,K", SHAPES, ids=lambda v: str(v)[:24])
 def test_products(counts, N, K, G, dt):
-    for sdt in (dt, torch.float32):
-        packed, scale = weights(len(counts), N, K, G, sdt, seed=N + K)
-        x = rows_of(sum(counts), K, dt)
-        got = int4.int4_grouped_mv(x, packed, scale, offsets(counts), G)
-        check(got, x, packed, scale, G, counts, False)
-        if N % 2 == 0:
-            got = int4.int4_grouped_mv(x, packed, scale, offsets(counts), G, silu=True)
-            check(got, x, packed, scale, G, counts, True)
+    packed, scale = weights(len(counts), N, K, G, dt, seed=N + K)
+    x = rows_of(sum(counts), K, dt)
+    got = int4.int4_grouped_mv(x, packed, scale, offsets(counts), G)
+    check(got, x, packed, scale, G, counts, False)
+    if N % 2 == 0:
+        got = int4.int4_grouped_mv(x, packed, scale, offsets(counts), G, silu=True)
+        check(got, x, packed, scale, G, counts, True)
 
 
 @pytest.mark.gpu
@@ -286,7 +285,7 @@ def test_refusals():
     for change, message in [
             (dict(x=x.float()), "bfloat16 or float16"), (dict(x=x[:, :32]), "twice"), (dict(x=x[0]), "rows, K"),
             (dict(w_packed=packed.to(torch.int8)), "uint8"), (dict(w_packed=packed.transpose(0, 1)), "contiguous"),
-            (dict(w_scale=scale.half()), "dtype or float32"), (dict(w_scale=scale[..., :1]), "ceil"),
+            (dict(w_scale=scale.float()), "x's dtype"), (dict(w_scale=scale[..., :1]), "ceil"),
             (dict(group_size=16), "32, 64 or 128"), (dict(group_size=64), "ceil"),
             (dict(expert_offsets=eo.long()), "int32"), (dict(expert_offsets=eo[:2]), "E \\+ 1"),
             (dict(expert_offsets=eo.cpu()), "device"), (dict(permuted_idx=pidx.long()), "permuted_idx"),
@@ -320,11 +319,11 @@ def test_c_argument_errors_before_any_cuda_call():
     lib = _lib.LIB
     one = ctypes.c_void_p(256)  # never read: every call below is refused first
 
-    def mv(x=one, stride=64, x_rows=4, dtype=0, pidx=None, topk=1, sdtype=0, G=32, E=2, rows=4, n=16, k=64, silu=0):
-        return lib.i8moe_int4_grouped_mv(x, stride, x_rows, dtype, pidx, topk, one, one, sdtype, G, one, E, rows, n, k,
-                                         silu, one, None)
+    def mv(x=one, stride=64, x_rows=4, dtype=0, pidx=None, topk=1, G=32, E=2, rows=4, n=16, k=64, silu=0):
+        return lib.i8moe_int4_grouped_mv(x, stride, x_rows, dtype, pidx, topk, one, one, G, one, E, rows, n, k, silu,
+                                         one, None)
 
-    for kw, message in [(dict(dtype=2, sdtype=2), "bfloat16"), (dict(sdtype=1), "w_scale"), (dict(G=16), "group_size"),
+    for kw, message in [(dict(dtype=2), "bfloat16"), (dict(G=16), "group_size"),
                         (dict(k=0), "K must"), (dict(k=48), "K must"), (dict(n=-1), "bad N"),
                         (dict(n=15, silu=1), "bad N"), (dict(E=-1), "n_expert"), (dict(E=4096), "n_expert"),
                         (dict(rows=-1), "n_rows"), (dict(rows=5), "fewer rows"), (dict(topk=0, pidx=one), "topk"),
