@@ -27,6 +27,7 @@ struct NormArgs {
   int weight_dtype;
   int64_t rows;
   int k;
+  float inv_k;  // 1 / k
   float eps;
   void* h;      // nullable
   void* y;      // nullable
@@ -45,6 +46,34 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v
   if (dtype == I8MOE_BF16) static_cast<__nv_bfloat16*>(p)[i] = Num<__nv_bfloat16>::from_f(v);
   else if (dtype == I8MOE_FP16) static_cast<__half*>(p)[i] = Num<__half>::from_f(v);
   else static_cast<float*>(p)[i] = v;
+}
+
+template <typename T, int kVec>
+__device__ __forceinline__ void load_weight(const void* w, int dtype, int i, float* out) {
+  if constexpr (sizeof(T) < 4) {
+    if (dtype != I8MOE_FP32) {
+      struct alignas(sizeof(T) * kVec) Raw {
+        T v[kVec];
+      };
+      const Raw raw = *reinterpret_cast<const Raw*>(static_cast<const T*>(w) + i);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) out[e] = Num<T>::to_f(raw.v[e]);
+      return;
+    }
+  }
+  if constexpr (kVec % 4 == 0) {
+#pragma unroll
+    for (int e = 0; e < kVec; e += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + i + e);
+      out[e] = f.x;
+      out[e + 1] = f.y;
+      out[e + 2] = f.z;
+      out[e + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) out[e] = static_cast<const float*>(w)[i + e];
+  }
 }
 
 // max that keeps NaN, so that a row without a finite norm gets a NaN scale
@@ -76,16 +105,135 @@ __device__ __forceinline__ float block_reduce(float v, float* s_part) {
   return v;
 }
 
-__device__ __forceinline__ int8_t to_int8(float y, float scale) {
-  // |y / scale| <= 127 but for its last bit, which rint takes back to 127; a
-  // NaN becomes 0 (the row's scale is NaN too)
-  return static_cast<int8_t>(__float2int_rn(__fdiv_rn(y, scale)));
+// rint(y * inv) as int8, for |y * inv| <= 127 up to its last bits: adding 1.5 *
+// 2^23 rounds to the nearest integer, ties to even, and leaves it in the low
+// bits.
+__device__ __forceinline__ int8_t to_int8(float y, float inv) {
+  return static_cast<int8_t>(__float_as_uint(fmaf(y, inv, 12582912.f)));
 }
 
-// Rows of any width and alignment: one CTA per row, which it reads up to
-// three times (sum of squares, absmax, output); the repeats hit L1/L2.
+// What the int8 values of a row are multiplied by: 127 over its largest |y|.
+// Non-finite rows give 0 and a mask of zeros, which makes their values 0.
+struct Int8Row {
+  float inv;
+  uint8_t mask;
+};
+__device__ __forceinline__ Int8Row int8_row(float largest) {
+  const bool finite = largest < __int_as_float(0x7f800000);
+  return {finite ? __fdividef(127.f, largest) : 0.f, static_cast<uint8_t>(finite ? 0xff : 0)};
+}
+
+// kVec elements that one thread reads or writes at once.
+template <typename T, int kVec>
+struct alignas(sizeof(T) * kVec) Pack {
+  T v[kVec];
+};
+
+// Rows in registers: blockDim.x threads hold a row, kPer packs each (a CTA has
+// several rows where a row takes less than a warp), so that it is read once,
+// and the sum of squares and the largest |h * weight| (from which the int8
+// scale follows, rstd being one factor of the row) are reduced together.  kVec
+// is 16 bytes' worth when width, strides and pointers allow it, else 1.
+// Bound by memory: 8192 x 2048 bf16 with a residual takes 26 us, 5.2 TB/s of
+// the 6.6 that a copy has; with two packs a thread 27, with four 30.
+template <typename T, int kVec, int kPer>
+__global__ void __launch_bounds__(1024) norm_row_kernel(NormArgs a) {
+  using P = Pack<T, kVec>;
+  __shared__ float s_sum[32], s_max[32];
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const int k = r < a.rows ? a.k : 0;
+  const int tid = threadIdx.x, stride = blockDim.x * kVec;
+  const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
+  const T* res = static_cast<const T*>(a.residual) + r * a.residual_stride;
+  P xv[kPer], rv[kPer];
+  float w[kPer][kVec];
+#pragma unroll
+  for (int p = 0; p < kPer; ++p) {
+    const int i = p * stride + tid * kVec;
+    if (i < k) {
+      xv[p] = *reinterpret_cast<const P*>(x + i);
+      if (a.residual) rv[p] = *reinterpret_cast<const P*>(res + i);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < kPer; ++p) {
+    const int i = p * stride + tid * kVec;
+    if (i < k) load_weight<T, kVec>(a.weight, a.weight_dtype, i, w[p]);
+  }
+  float h[kPer][kVec];
+  float ss = 0.f, m = 0.f;
+#pragma unroll
+  for (int p = 0; p < kPer; ++p) {
+    const int i = p * stride + tid * kVec;
+    if (i < k) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        h[p][e] = Num<T>::to_f(xv[p].v[e]);
+        if (a.residual) h[p][e] += Num<T>::to_f(rv[p].v[e]);
+        ss = fmaf(h[p][e], h[p][e], ss);
+        m = max_nan(m, fabsf(h[p][e] * w[p][e]));
+      }
+      if (a.h) {
+        P o;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) o.v[e] = Num<T>::from_f(h[p][e]);
+        *reinterpret_cast<P*>(static_cast<T*>(a.h) + r * a.k + i) = o;
+      }
+    }
+  }
+  for (int o = min(32, static_cast<int>(blockDim.x)) >> 1; o > 0; o >>= 1) {
+    ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  }
+  if (blockDim.x > 32) {  // one row
+    if ((tid & 31) == 0) {
+      s_sum[tid >> 5] = ss;
+      s_max[tid >> 5] = m;
+    }
+    __syncthreads();
+    const bool on = (tid & 31) < (blockDim.x >> 5);
+    ss = on ? s_sum[tid & 31] : 0.f;
+    m = on ? s_max[tid & 31] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    }
+  }
+  const float rstd = rsqrtf(fmaf(ss, a.inv_k, a.eps));
+  const float largest = max_nan(m * rstd, 1e-10f);
+  const Int8Row row = int8_row(largest);
+  if (tid == 0 && k > 0) {
+    if (a.rstd) a.rstd[r] = rstd;
+    if (a.q) a.scale[r] = largest / 127.f;
+  }
+#pragma unroll
+  for (int p = 0; p < kPer; ++p) {
+    const int i = p * stride + tid * kVec;
+    if (i < k) {
+      float y[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) y[e] = h[p][e] * rstd * w[p][e];
+      if (a.y) {
+        P o;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) o.v[e] = Num<T>::from_f(y[e]);
+        *reinterpret_cast<P*>(static_cast<T*>(a.y) + r * a.k + i) = o;
+      }
+      if (a.q) {
+        Pack<int8_t, kVec> o;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) o.v[e] = to_int8(y[e], row.inv) & row.mask;
+        *reinterpret_cast<Pack<int8_t, kVec>*>(a.q + r * a.k + i) = o;
+      }
+    }
+  }
+}
+
+// Rows too wide for the registers of a CTA: read up to three times (sum of
+// squares, absmax, output); the repeats hit L1/L2.
 template <typename T>
-__global__ void __launch_bounds__(256) norm_any_kernel(NormArgs a) {
+__global__ void __launch_bounds__(256) norm_wide_kernel(NormArgs a) {
   __shared__ float s_part[8];
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
@@ -101,22 +249,23 @@ __global__ void __launch_bounds__(256) norm_any_kernel(NormArgs a) {
       ss = fmaf(h, h, ss);
     }
     ss = block_reduce<Sum>(ss, s_part);
-    const float rstd = __frsqrt_rn(ss / static_cast<float>(a.k) + a.eps);
+    const float rstd = rsqrtf(fmaf(ss, a.inv_k, a.eps));
     if (a.rstd && threadIdx.x == 0) a.rstd[r] = rstd;
-    float scale = 0.f;
+    Int8Row row{};
     if (a.q) {
       float m = 0.f;
       for (int i = threadIdx.x; i < a.k; i += blockDim.x)
         m = max_nan(m, fabsf(h_at(i) * rstd * load_any(a.weight, a.weight_dtype, i)));
-      scale = max_nan(block_reduce<MaxNan>(m, s_part), 1e-10f) / 127.f;
-      if (threadIdx.x == 0) a.scale[r] = scale;
+      const float largest = max_nan(block_reduce<MaxNan>(m, s_part), 1e-10f);
+      row = int8_row(largest);
+      if (threadIdx.x == 0) a.scale[r] = largest / 127.f;
     }
     for (int i = threadIdx.x; i < a.k; i += blockDim.x) {
       const float h = h_at(i);
       const float y = h * rstd * load_any(a.weight, a.weight_dtype, i);
       if (a.h) static_cast<T*>(a.h)[r * a.k + i] = Num<T>::from_f(h);
       if (a.y) static_cast<T*>(a.y)[r * a.k + i] = Num<T>::from_f(y);
-      if (a.q) a.q[r * a.k + i] = to_int8(y, scale);
+      if (a.q) a.q[r * a.k + i] = to_int8(y, row.inv) & row.mask;
     }
   }
 }
@@ -131,17 +280,192 @@ struct NormGradArgs {
   const float* rstd;
   int64_t rows;
   int k;
+  float inv_k;  // 1 / k
   void* dx;
   float* part;  // [n_part, k], nullable: no weight gradient is wanted
   int n_part;
 };
 
-// Partial sums of the weight's gradient that a backward pass writes (one row
-// of k each) before they are added up in a fixed order.
+constexpr int kGradThreads = 512;
+template <int kPer>
+constexpr int kGradStages = kPer > 2 ? 2 : 3;  // rows of a group in shared memory
+template <int kVec, int kPer>
+constexpr int kGradCtas = kPer <= (kVec == 1 ? 4 : 1) ? 2 : 1;  // resident on an SM
+// The most CTAs of a backward pass, and partial sums of the weight's gradient
+// that it writes (one row of k each) before they are added up.
 constexpr int kNormParts = 296;
 
+// The kThreads threads of a group hold a row's columns, kPer packs each, for
+// all rows that the group takes, and add up their share of the weight's
+// gradient in registers.  Rows come through a ring of kGradStages in shared
+// memory, of which every thread reads what it copied itself, so that the next
+// rows are on their way during a row's one reduction (one barrier of the
+// group; the halves of s_part take turns) without holding registers: with the
+// next row in registers instead, the default size took 48 us, spills and all.
+// Single elements (kVec 1) do wait in registers, of which they take few.  A
+// CTA's groups meet at its end.  The grid is what is resident at once.
+template <typename T, int kVec, int kPer, int kThreads, bool kWeight>
+__global__ void __launch_bounds__(kGradThreads, kGradCtas<kVec, kPer>)
+    norm_grad_row_kernel(NormGradArgs a) {
+  using P = Pack<T, kVec>;
+  constexpr bool kRing = kVec > 1;
+  constexpr int kGroups = kGradThreads / kThreads, kWarps = kThreads / 32;
+  constexpr int kStages = kGradStages<kPer>;
+  extern __shared__ uint4 s_ring[];  // [stage][h, dy, dh][kPer][thread of the CTA]
+  __shared__ float s_part[2][kGradThreads / 32];
+  const int group = threadIdx.x / kThreads, tid = threadIdx.x % kThreads;
+  const int lane = tid & 31;
+  const int64_t rows_at_once = static_cast<int64_t>(gridDim.x) * kGroups;
+  int64_t r = static_cast<int64_t>(group) * gridDim.x + blockIdx.x;
+  auto row_of = [&](int which, int64_t row) {
+    return which == 0   ? static_cast<const T*>(a.h) + row * a.h_stride
+           : which == 1 ? static_cast<const T*>(a.dy) + row * a.dy_stride
+                        : static_cast<const T*>(a.dh) + row * a.dh_stride;
+  };
+  auto ring = [&](int stage, int which, int p) {
+    return s_ring + ((stage * 3 + which) * kPer + p) * kGradThreads + threadIdx.x;
+  };
+  auto copy = [&](int64_t row, int stage) {
+    if (row < a.rows)
+#pragma unroll
+      for (int which = 0; which < 3; ++which)
+        if (which < 2 || a.dh)
+#pragma unroll
+          for (int p = 0; p < kPer; ++p) {
+            const int i = (p * kThreads + tid) * kVec;
+            if (i < a.k)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                               smem_u32(ring(stage, which, p))),
+                           "l"(row_of(which, row) + i)
+                           : "memory");
+          }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  P now[kRing ? 1 : 3][kPer], next[kRing ? 1 : 3][kPer];
+  auto load = [&](int64_t row) {
+#pragma unroll
+    for (int which = 0; which < 3; ++which)
+#pragma unroll
+      for (int p = 0; p < kPer; ++p) {
+        const int i = (p * kThreads + tid) * kVec;
+        if (i < a.k && (which < 2 || a.dh))
+          next[kRing ? 0 : which][p] = *reinterpret_cast<const P*>(row_of(which, row) + i);
+      }
+  };
+  auto get = [&](int stage, int which, int p) {
+    if constexpr (kRing) return *reinterpret_cast<const P*>(ring(stage, which, p));
+    else return now[which][p];
+  };
+
+  if constexpr (kRing) {
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) copy(r + s * rows_at_once, s);
+  } else if (r < a.rows) {
+    load(r);
+  }
+  float w[kPer][kVec], dw[kPer][kVec];
+#pragma unroll
+  for (int p = 0; p < kPer; ++p) {
+    const int i = (p * kThreads + tid) * kVec;
+    if (i < a.k) load_weight<T, kVec>(a.weight, a.weight_dtype, i, w[p]);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) dw[p][e] = 0.f;
+  }
+  float rstd_next = r < a.rows ? a.rstd[r] : 0.f;
+  for (int turn = 0, stage = 0; r < a.rows; turn ^= 1) {
+    const float rstd = rstd_next;
+    if (r + rows_at_once < a.rows) rstd_next = a.rstd[r + rows_at_once];
+    if constexpr (kRing) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    } else {
+#pragma unroll
+      for (int which = 0; which < 3; ++which)
+#pragma unroll
+        for (int p = 0; p < kPer; ++p) now[which][p] = next[which][p];
+      if (r + rows_at_once < a.rows) load(r + rows_at_once);
+    }
+    float dot = 0.f;  // of dy * weight and h
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      const int i = (p * kThreads + tid) * kVec;
+      if (i < a.k) {
+        const P h = get(stage, 0, p), g = get(stage, 1, p);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const float hf = Num<T>::to_f(h.v[e]), gf = Num<T>::to_f(g.v[e]);
+          if constexpr (kWeight) dw[p][e] = fmaf(gf * rstd, hf, dw[p][e]);
+          dot = fmaf(gf * w[p][e], hf, dot);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if constexpr (kWarps > 1) {
+      float* part = s_part[turn] + group * kWarps;
+      if (lane == 0) part[tid >> 5] = dot;
+      asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(kThreads) : "memory");
+      dot = part[lane % kWarps];
+#pragma unroll
+      for (int o = kWarps / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    }
+    // dx = rstd * (a - n * mean(a * n)) with n = h * rstd
+    const float back = -(rstd * rstd) * (rstd * (dot * a.inv_k));
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      const int i = (p * kThreads + tid) * kVec;
+      if (i < a.k) {
+        const P h = get(stage, 0, p), g = get(stage, 1, p);
+        P o, add;
+        if (a.dh) add = get(stage, 2, p);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          float d = Num<T>::to_f(h.v[e]) * back;
+          d = fmaf(Num<T>::to_f(g.v[e]) * w[p][e], rstd, d);
+          if (a.dh) d += Num<T>::to_f(add.v[e]);
+          o.v[e] = Num<T>::from_f(d);
+        }
+        *reinterpret_cast<P*>(static_cast<T*>(a.dx) + r * a.k + i) = o;
+      }
+    }
+    if constexpr (kRing) {
+      copy(r + kStages * rows_at_once, stage);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    r += rows_at_once;
+  }
+  if constexpr (kWeight) {
+    float* s_dw = reinterpret_cast<float*>(s_ring);  // [group - 1][kPer * kVec][kThreads]
+    if constexpr (kGroups > 1) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncthreads();
+      if (group > 0)
+#pragma unroll
+        for (int p = 0; p < kPer; ++p)
+#pragma unroll
+          for (int e = 0; e < kVec; ++e)
+            s_dw[((group - 1) * kPer * kVec + p * kVec + e) * kThreads + tid] = dw[p][e];
+      __syncthreads();
+      if (group > 0) return;
+    }
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      const int i = (p * kThreads + tid) * kVec;
+      if (i < a.k)
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          float v = dw[p][e];
+          for (int o = 0; o < kGroups - 1; ++o)
+            v += s_dw[(o * kPer * kVec + p * kVec + e) * kThreads + tid];
+          a.part[static_cast<int64_t>(blockIdx.x) * a.k + i + e] = v;
+        }
+    }
+  }
+}
+
+// Rows too wide for the registers of a CTA: read twice, and once more for the
+// weight's gradient.
 template <typename T>
-__global__ void __launch_bounds__(256) norm_grad_any_kernel(NormGradArgs a) {
+__global__ void __launch_bounds__(256) norm_grad_wide_kernel(NormGradArgs a) {
   __shared__ float s_part[8];
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* h = static_cast<const T*>(a.h) + r * a.h_stride;
@@ -152,7 +476,7 @@ __global__ void __launch_bounds__(256) norm_grad_any_kernel(NormGradArgs a) {
     for (int i = threadIdx.x; i < a.k; i += blockDim.x)
       dot += Num<T>::to_f(dy[i]) * load_any(a.weight, a.weight_dtype, i) *
              (Num<T>::to_f(h[i]) * rstd);
-    const float mean = block_reduce<Sum>(dot, s_part) / static_cast<float>(a.k);
+    const float mean = block_reduce<Sum>(dot, s_part) * a.inv_k;
     for (int i = threadIdx.x; i < a.k; i += blockDim.x) {
       const float n = Num<T>::to_f(h[i]) * rstd;
       const float g = Num<T>::to_f(dy[i]) * load_any(a.weight, a.weight_dtype, i);
@@ -175,32 +499,113 @@ __global__ void __launch_bounds__(256) norm_weight_part_kernel(NormGradArgs a) {
   a.part[static_cast<int64_t>(blockIdx.y) * a.k + i] = s;
 }
 
-__global__ void __launch_bounds__(256) norm_weight_sum_kernel(const float* part, int n_part, int k,
-                                                              void* dweight, int dtype) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= k) return;
-  float s = 0.f;
-  for (int p = 0; p < n_part; ++p) s += part[static_cast<int64_t>(p) * k + i];
-  store_any(dweight, dtype, i, s);
+// Adds up the partial sums: 32 columns a CTA, its 32 warps a share of the parts
+// each, in a fixed order.
+__global__ void __launch_bounds__(1024) norm_weight_sum_kernel(const float* part, int n_part, int k,
+                                                               void* dweight, int dtype) {
+  __shared__ float s[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int i = blockIdx.x * 32 + lane;
+  float v = 0.f;
+  if (i < k)
+    for (int p = warp; p < n_part; p += 32) v += part[static_cast<int64_t>(p) * k + i];
+  s[warp][lane] = v;
+  __syncthreads();
+  v = s[lane][warp];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int c = blockIdx.x * 32 + warp;
+  if (lane == 0 && c < k) store_any(dweight, dtype, c, v);
 }
 
 bool float_dtype(int d) { return d == I8MOE_BF16 || d == I8MOE_FP16 || d == I8MOE_FP32; }
 
-template <typename T>
-int launch_norm(const NormArgs& a, cudaStream_t st) {
-  const int sms = num_sms(current_device());
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, sms * 8));
-  norm_any_kernel<T><<<grid, 256, 0, st>>>(a);
-  return check_launch("rms_norm");
+uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+template <typename T, int kVec, int kPer>
+void launch_norm_row(const NormArgs& a, cudaStream_t st) {
+  const int need = (a.k + kVec * kPer - 1) / (kVec * kPer);
+  int x = 1;
+  while (x < 32 && x < need) x *= 2;
+  if (need > 32) x = (need + 31) / 32 * 32;
+  const int y = x <= 32 ? 128 / x : 1;
+  norm_row_kernel<T, kVec, kPer>
+      <<<static_cast<unsigned>((a.rows + y - 1) / y), dim3(x, y), 0, st>>>(a);
+}
+
+// One pack a thread while that makes no CTA of more than 512 threads; elements
+// one by one come eight to a thread (4096 x 2047 bf16: 33 us with four, 41
+// with two).
+template <typename T, int kVec>
+bool launch_norm_rows(const NormArgs& a, cudaStream_t st) {
+  if (kVec == 1 && a.k <= 8 * 1024) launch_norm_row<T, 1, 8>(a, st);
+  else if (kVec > 1 && a.k <= kVec * 512) launch_norm_row<T, kVec, 1>(a, st);
+  else if (kVec > 1 && a.k <= kVec * 2 * 1024) launch_norm_row<T, kVec, 2>(a, st);
+  else return false;
+  return true;
 }
 
 template <typename T>
-int launch_norm_grad(const NormGradArgs& a, cudaStream_t st) {
-  const int sms = num_sms(current_device());
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, sms * 8));
-  norm_grad_any_kernel<T><<<grid, 256, 0, st>>>(a);
-  if (a.part)
-    norm_weight_part_kernel<T><<<dim3((a.k + 255) / 256, a.n_part), 256, 0, st>>>(a);
+int launch_norm(const NormArgs& a, cudaStream_t st) {
+  constexpr int kVec = 16 / sizeof(T);
+  const bool packs =
+      a.k % kVec == 0 && a.x_stride % kVec == 0 && (!a.residual || a.residual_stride % kVec == 0) &&
+      (bits(a.x) | bits(a.residual) | bits(a.weight) | bits(a.h) | bits(a.y)) % 16 == 0 &&
+      bits(a.q) % 8 == 0;
+  if (!(packs ? launch_norm_rows<T, kVec>(a, st) : launch_norm_rows<T, 1>(a, st))) {
+    const int sms = num_sms(current_device());
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, sms * 8));
+    norm_wide_kernel<T><<<grid, 256, 0, st>>>(a);
+  }
+  return check_launch("rms_norm");
+}
+
+template <typename T, int kVec, int kPer, int kThreads>
+int launch_norm_grad_kernel(NormGradArgs& a, cudaStream_t st) {
+  const int64_t groups = kGradThreads / kThreads;
+  const int64_t most = int64_t(num_sms(current_device())) * kGradCtas<kVec, kPer>;
+  a.n_part = static_cast<int>(
+      std::min({(a.rows + groups - 1) / groups, most, int64_t(kNormParts)}));
+  constexpr int kRing = kVec > 1 ? kGradStages<kPer> * 3 * kPer * kGradThreads * 16 : 0;
+  constexpr int kMeet = (kGradThreads / kThreads - 1) * kPer * kVec * kThreads * 4;
+  constexpr int kSmem = kRing > kMeet ? kRing : kMeet;
+  auto kernel = a.part ? norm_grad_row_kernel<T, kVec, kPer, kThreads, true>
+                       : norm_grad_row_kernel<T, kVec, kPer, kThreads, false>;
+  if (kSmem > 48 * 1024)
+    I8_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  kernel<<<a.n_part, kGradThreads, kSmem, st>>>(a);
+  return check_launch("rms_norm_backward");
+}
+
+// Widths that fit a CTA's registers; `*wide` says that this one does not.
+template <typename T, int kVec>
+int launch_norm_grad_rows(NormGradArgs& a, cudaStream_t st, bool* wide) {
+  constexpr int kMost = kVec == 1 ? 8 : kVec == 4 ? 4 : 2;  // what the registers hold
+  const int packs = (a.k + kVec - 1) / kVec;
+  if (packs <= 32) return launch_norm_grad_kernel<T, kVec, 1, 32>(a, st);
+  if (packs <= 64) return launch_norm_grad_kernel<T, kVec, 1, 64>(a, st);
+  if (packs <= 128) return launch_norm_grad_kernel<T, kVec, 1, 128>(a, st);
+  if (packs <= 256) return launch_norm_grad_kernel<T, kVec, 1, 256>(a, st);
+  if (packs <= 512) return launch_norm_grad_kernel<T, kVec, 1, 512>(a, st);
+  if (packs <= 1024) return launch_norm_grad_kernel<T, kVec, 2, 512>(a, st);
+  if (packs <= 512 * kMost) return launch_norm_grad_kernel<T, kVec, kMost, 512>(a, st);
+  *wide = true;
+  return I8MOE_OK;
+}
+
+template <typename T>
+int launch_norm_grad(NormGradArgs& a, cudaStream_t st) {
+  constexpr int kVec = 16 / sizeof(T);
+  const bool packs = a.k % kVec == 0 && a.h_stride % kVec == 0 && a.dy_stride % kVec == 0 &&
+                     (!a.dh || a.dh_stride % kVec == 0) &&
+                     (bits(a.h) | bits(a.dy) | bits(a.dh) | bits(a.weight) | bits(a.dx)) % 16 == 0;
+  bool wide = false;
+  const int rc = packs ? launch_norm_grad_rows<T, kVec>(a, st, &wide)
+                       : launch_norm_grad_rows<T, 1>(a, st, &wide);
+  if (!wide) return rc;
+  a.n_part = static_cast<int>(std::min<int64_t>(a.rows, kNormParts));
+  norm_grad_wide_kernel<T><<<a.n_part, 256, 0, st>>>(a);
+  if (a.part) norm_weight_part_kernel<T><<<dim3((a.k + 255) / 256, a.n_part), 256, 0, st>>>(a);
   return check_launch("rms_norm_backward");
 }
 
@@ -218,7 +623,8 @@ int i8moe_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_
   I8_REQUIRE(float_dtype(dtype), "rms_norm: unsupported dtype");
   I8_REQUIRE(weight_dtype == dtype || weight_dtype == I8MOE_FP32,
              "rms_norm: weight must have the rows' dtype or float32");
-  I8_REQUIRE(n_rows >= 0 && n_hidden >= 1 && n_hidden < (int64_t(1) << 31) - 1024,
+  I8_REQUIRE(n_rows >= 0 && n_rows < (int64_t(1) << 31) && n_hidden >= 1 &&
+                 n_hidden < (int64_t(1) << 31) - 1024,
              "rms_norm: bad n_rows / n_hidden");
   I8_REQUIRE(eps >= 0.f && eps < 3.0e38f, "rms_norm: eps must be finite and not negative");
   if (n_rows == 0) return I8MOE_OK;
@@ -228,7 +634,8 @@ int i8moe_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_
   I8_REQUIRE(y != nullptr || q != nullptr, "rms_norm: no output given");
   I8_REQUIRE(x != nullptr && weight != nullptr, "rms_norm: x and weight must be given");
   NormArgs a{x, residual, weight, x_stride, residual_stride, weight_dtype, n_rows,
-             static_cast<int>(n_hidden), eps, residual_out, y, rstd, q, q_scale};
+             static_cast<int>(n_hidden), 1.f / static_cast<float>(n_hidden), eps, residual_out, y,
+             rstd, q, q_scale};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == I8MOE_BF16) return launch_norm<__nv_bfloat16>(a, st);
   if (dtype == I8MOE_FP16) return launch_norm<__half>(a, st);
@@ -260,21 +667,21 @@ int i8moe_rms_norm_backward(const void* dy, int64_t dy_stride, const void* resid
   I8_REQUIRE(dy && h && weight && rstd && dx,
              "rms_norm_backward: dy, h, weight, rstd and dx must be given");
   NormGradArgs a{dy, residual_grad, h, weight, dy_stride, residual_grad_stride, h_stride,
-                 weight_dtype, rstd, n_rows, static_cast<int>(n_hidden), dx, nullptr, 0};
+                 weight_dtype, rstd, n_rows, static_cast<int>(n_hidden),
+                 1.f / static_cast<float>(n_hidden), dx, nullptr, 0};
   if (dweight) {
     I8_REQUIRE(workspace != nullptr && workspace_bytes >= i8moe_rms_norm_backward_workspace_size(
                                                               n_rows, n_hidden),
                "rms_norm_backward: the workspace is too small");
     a.part = static_cast<float*>(workspace);
-    a.n_part = static_cast<int>(std::min<int64_t>(n_rows, kNormParts));
   }
   int rc;
   if (dtype == I8MOE_BF16) rc = launch_norm_grad<__nv_bfloat16>(a, st);
   else if (dtype == I8MOE_FP16) rc = launch_norm_grad<__half>(a, st);
   else rc = launch_norm_grad<float>(a, st);
   if (rc != I8MOE_OK || !dweight) return rc;
-  norm_weight_sum_kernel<<<(a.k + 255) / 256, 256, 0, st>>>(a.part, a.n_part, a.k, dweight,
-                                                            weight_dtype);
+  norm_weight_sum_kernel<<<(a.k + 31) / 32, 1024, 0, st>>>(a.part, a.n_part, a.k, dweight,
+                                                           weight_dtype);
   return check_launch("rms_norm_backward: weight");
 }
 
