@@ -1,4 +1,5 @@
-"""Build libi8moe.so in-tree with nvcc for sm_100a.
+"""Build libi8moe.so in-tree with nvcc for sm_100a, and its compiled torch
+binding _torch_ops.so with the host compiler.
 
     python int8blockwisegemm_b200/_build.py [--force] [--verbose]
 
@@ -24,6 +25,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libi8moe.so"
+TORCH_OPS = PKG / "_torch_ops.so"
 INCLUDE = ROOT / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -63,10 +65,41 @@ def _compile(src: Path, force: bool, verbose: bool, extra: list[str]) -> Path:
     return obj
 
 
+def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
+    """The torch binding (csrc/torch_ops.cpp, host code only)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    src = CSRC / "torch_ops.cpp"
+    header = INCLUDE / "i8moe.h"
+    if (not force and TORCH_OPS.exists()
+            and TORCH_OPS.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime)):
+        return TORCH_OPS
+    cuda = Path(nvcc()).resolve().parent.parent
+    includes = [INCLUDE, *cpp_extension.include_paths(), cuda / "include",
+                sysconfig.get_paths()["include"]]
+    torch_lib = Path(torch.__file__).parent / "lib"
+    tmp = TORCH_OPS.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(f"-isystem{p}" for p in includes), str(src), "-o", str(tmp), f"-L{torch_lib}",
+           "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, TORCH_OPS)
+    return TORCH_OPS
+
+
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> Path:
     BUILD.mkdir(exist_ok=True)
     extra = list(extra or [])
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        ops = ex.submit(build_torch_ops, force, verbose)
         objs = list(ex.map(lambda s: _compile(s, force, verbose, extra), sources()))
     newest = max(o.stat().st_mtime for o in objs)
     if force or not LIB.exists() or LIB.stat().st_mtime < newest:
@@ -78,6 +111,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
+    ops.result()
     return LIB
 
 

@@ -101,6 +101,23 @@ def _load():
 LIB = _load()
 
 
+def _load_torch_ops():
+    """The compiled torch binding of the operators with gradients or single-
+    token forms, on the functions of the library that was loaded."""
+    try:
+        from . import _torch_ops
+    except ImportError as exc:
+        raise RuntimeError(
+            "Cannot load _torch_ops.so.\n"
+            "Build it first:  python int8blockwisegemm_b200/_build.py") from exc
+    _torch_ops.bind({name: ctypes.cast(getattr(LIB, name), c_void_p).value
+                     for name in PROTOTYPES})
+    return _torch_ops
+
+
+TORCH_OPS = _load_torch_ops()
+
+
 def last_error() -> str:
     msg = LIB.i8moe_last_error()
     return msg.decode() if msg else ""

@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import BF16, FP16, FP32, launch
+from ._lib import BF16, FP16, FP32, TORCH_OPS, launch
 from .permute import moe_route_for_gemm, moe_unpermute
 
 _DT = {torch.bfloat16: BF16, torch.float16: FP16, torch.float32: FP32}
@@ -56,49 +56,8 @@ def int4_grouped_mv(x, w_packed, w_scale, expert_offsets, group_size: int = 128,
     Returns ``out`` [rows, N] (N/2 with silu) in x's type, allocated when not
     given; rows outside every expert keep what it held.  Sums are fp32,
     rounded once."""
-    _check(x.is_cuda and x.dim() == 2, "int4_grouped_mv: x must be a CUDA tensor [rows, K]")
-    _check(x.dtype in (torch.bfloat16, torch.float16),
-           "int4_grouped_mv: x must be bfloat16 or float16")
-    dev = x.device
-    _check(w_packed.dtype == torch.uint8 and w_packed.dim() == 3 and w_packed.is_contiguous()
-           and w_packed.device == dev,
-           "int4_grouped_mv: w_packed must be contiguous uint8 [E, N, K/2] on x's device")
-    E, N, half = w_packed.shape
-    K = 2 * half
-    _check(group_size in (32, 64, 128), "int4_grouped_mv: group_size must be 32, 64 or 128")
-    _check(x.size(1) == K, "int4_grouped_mv: x.shape[1] must be twice w_packed.shape[2]")
-    _check(K >= 32 and K % 32 == 0, "int4_grouped_mv: K must be positive and divisible by 32")
-    _check(w_scale.dtype == x.dtype, "int4_grouped_mv: w_scale must have x's dtype")
-    _check(w_scale.shape == (E, N, -(-K // group_size)) and w_scale.is_contiguous()
-           and w_scale.device == dev,
-           "int4_grouped_mv: w_scale must be contiguous [E, N, ceil(K / group_size)] on x's device")
-    _check(expert_offsets.dtype == torch.int32 and expert_offsets.shape == (E + 1,)
-           and expert_offsets.is_contiguous() and expert_offsets.device == dev,
-           "int4_grouped_mv: expert_offsets must be contiguous int32 [E + 1] on x's device")
-    _check(not silu or N % 2 == 0, "int4_grouped_mv: N must be even with silu")
-    rows = x.size(0)
-    if permuted_idx is not None:
-        _check(permuted_idx.dtype == torch.int32 and permuted_idx.dim() == 1
-               and permuted_idx.is_contiguous() and permuted_idx.device == dev,
-               "int4_grouped_mv: permuted_idx must be contiguous int32 [rows] on x's device")
-        _check(topk >= 1, "int4_grouped_mv: topk must be positive")
-        rows = permuted_idx.size(0)
-    n_out = N // 2 if silu else N
-    if out is None:
-        out = torch.empty((rows, n_out), dtype=x.dtype, device=dev)
-    else:
-        _check(out.dtype == x.dtype and out.shape == (rows, n_out) and out.is_contiguous()
-               and out.device == dev,
-               "int4_grouped_mv: out must be contiguous [rows, N (N/2 with silu)] of x's dtype "
-               "on x's device")
-    if x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.stride(0) < K or x.data_ptr() % 16 != 0:
-        x = x.contiguous() if x.data_ptr() % 16 == 0 else x.clone(
-            memory_format=torch.contiguous_format)
-    launch("i8moe_int4_grouped_mv", dev, x.data_ptr(), K if x.size(0) < 2 else x.stride(0),
-           x.size(0), _DT[x.dtype], permuted_idx.data_ptr() if permuted_idx is not None else None,
-           topk, w_packed.data_ptr(), w_scale.data_ptr(), group_size,
-           expert_offsets.data_ptr(), E, rows, N, K, 1 if silu else 0, out.data_ptr())
-    return out
+    return TORCH_OPS.int4_grouped_mv(x, w_packed, w_scale, expert_offsets, group_size, permuted_idx,
+                                     topk, silu, out)
 
 
 def run_int4_moe(output, hidden_states, w1_packed, w1_scale, w2_packed, w2_scale, topk_ids,

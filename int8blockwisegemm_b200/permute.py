@@ -5,12 +5,9 @@ with the sentinel n_token*topk, token_expert_indices is arange."""
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
-from ._lib import BF16, FP16, FP32, LIB, launch
-
-_DT = {torch.bfloat16: BF16, torch.float16: FP16, torch.float32: FP32}
+from ._lib import TORCH_OPS
 
 
 def _alloc(n_token: int, topk: int, n_local_expert: int, device):
@@ -154,136 +151,6 @@ def moe_unpermute(out, permuted_hidden_states, topk_weights, inv_permuted_idx,
 # same leaves before capturing a backward pass.
 # ---------------------------------------------------------------------------
 
-def _check(cond: bool, msg: str) -> None:
-    if not cond:
-        raise RuntimeError(msg)
-
-
-def _check_rows(what: str, name: str, t) -> None:
-    _check(t.is_cuda and t.dim() == 2, f"{what}: {name} must be a CUDA tensor [rows, hidden]")
-    _check(t.dtype in _DT, f"{what}: {name} must be bfloat16, float16 or float32")
-    _check(t.size(1) * t.element_size() % 16 == 0,
-           f"{what}: hidden row must be a multiple of 16 bytes")
-
-
-def _check_maps(what: str, inv, eft, rows: int, device) -> None:
-    _check(inv.dtype == torch.int32 and inv.is_contiguous() and inv.device == device
-           and inv.numel() == rows,
-           f"{what}: inv_permuted_idx must be contiguous int32 with n_token * topk elements")
-    if eft is not None:
-        _check(eft.dtype == torch.int64 and eft.is_contiguous() and eft.device == device
-               and eft.dim() == 1 and eft.numel() >= 1,
-               f"{what}: expert_first_token_offset must be contiguous int64 [n_local_expert + 1]")
-
-
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` contiguous and 16-byte aligned, copied when it is not."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _eft_args(eft):
-    return (None, 0) if eft is None else (eft.data_ptr(), eft.numel() - 1)
-
-
-def moe_permute_backward(permuted_grad, inv_permuted_idx, expert_first_token_offset, n_token: int,
-                         topk: int):
-    """Gradient of the row copy: [n_token, hidden], the sum of each token's
-    rows of ``permuted_grad`` that belong to local experts."""
-    what = "moe_permute_backward"
-    _check_rows(what, "permuted_grad", permuted_grad)
-    _check(n_token >= 0 and topk >= 1 and permuted_grad.size(0) == n_token * topk,
-           f"{what}: permuted_grad must have n_token * topk rows")
-    dev = permuted_grad.device
-    _check_maps(what, inv_permuted_idx, expert_first_token_offset, n_token * topk, dev)
-    g = _aligned(permuted_grad)
-    out = torch.empty((n_token, g.size(1)), dtype=g.dtype, device=dev)
-    launch("i8moe_moe_permute_backward", dev, g.data_ptr(), _DT[g.dtype],
-           inv_permuted_idx.data_ptr(), *_eft_args(expert_first_token_offset), n_token, topk,
-           g.size(1), out.data_ptr())
-    return out
-
-
-def moe_unpermute_backward(out_grad, permuted_hidden_states, topk_weights, inv_permuted_idx,
-                           expert_first_token_offset=None):
-    """Gradients of ``moe_unpermute``: (of permuted_hidden_states, of
-    topk_weights in fp32); zero for rows of no local expert."""
-    what = "moe_unpermute_backward"
-    _check_rows(what, "permuted_hidden_states", permuted_hidden_states)
-    dev = permuted_hidden_states.device
-    _check(topk_weights.dim() == 2 and topk_weights.dtype == torch.float32
-           and topk_weights.device == dev, f"{what}: topk_weights must be float32 [n_token, topk]")
-    n_token, topk = topk_weights.shape
-    _check(topk >= 1 and permuted_hidden_states.size(0) == n_token * topk,
-           f"{what}: permuted_hidden_states must have n_token * topk rows")
-    _check(out_grad.shape == (n_token, permuted_hidden_states.size(1))
-           and out_grad.dtype == permuted_hidden_states.dtype and out_grad.device == dev,
-           f"{what}: out_grad must be [n_token, hidden] of permuted_hidden_states' dtype")
-    _check_maps(what, inv_permuted_idx, expert_first_token_offset, n_token * topk, dev)
-    g, y, w = _aligned(out_grad), _aligned(permuted_hidden_states), topk_weights.contiguous()
-    dy = torch.empty_like(y)
-    dw = torch.empty_like(w)
-    launch("i8moe_moe_unpermute_backward", dev, g.data_ptr(), y.data_ptr(), _DT[y.dtype],
-           w.data_ptr(), inv_permuted_idx.data_ptr(), *_eft_args(expert_first_token_offset),
-           n_token, topk, y.size(1), dy.data_ptr(), dw.data_ptr())
-    return dy, dw
-
-
-def _sort_rows(x, ids, emap, n_expert, n_local_expert):
-    T, topk = ids.shape
-    dev, rows = x.device, T * topk
-    eft = torch.empty(n_local_expert + 1, dtype=torch.int64, device=dev)
-    inv = torch.empty(rows, dtype=torch.int32, device=dev)
-    pidx = torch.empty(rows, dtype=torch.int32, device=dev)
-    out = torch.empty((rows, x.size(1)), dtype=x.dtype, device=dev)
-    nbytes = LIB.i8moe_route_workspace_size(rows, n_expert)
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    launch("i8moe_moe_permute_metadata", dev, ids.data_ptr(), None,
-           emap.data_ptr() if emap is not None else None, T, topk, n_expert, n_local_expert,
-           eft.data_ptr(), inv.data_ptr(), pidx.data_ptr(), ws.data_ptr(), nbytes)
-    launch("i8moe_moe_scatter_rows", dev, x.data_ptr(), _DT[x.dtype], inv.data_ptr(),
-           eft.data_ptr(), n_local_expert, T, topk, x.size(1), out.data_ptr())
-    return out, eft, inv, pidx
-
-
-class _SortRows(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, ids, emap, n_expert, n_local_expert):
-        out, eft, inv, pidx = _sort_rows(x, ids, emap, n_expert, n_local_expert)
-        ctx.save_for_backward(eft, inv)
-        ctx.tokens = tuple(ids.shape)
-        ctx.mark_non_differentiable(eft, inv, pidx)
-        ctx.set_materialize_grads(False)
-        return out, eft, inv, pidx
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad, *_):
-        if grad is None:
-            return (None,) * 5
-        eft, inv = ctx.saved_tensors
-        return moe_permute_backward(grad, inv, eft, *ctx.tokens), None, None, None, None
-
-
-class _ReturnRows(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, rows, weights, inv, eft):
-        out = torch.empty((weights.size(0), rows.size(1)), dtype=rows.dtype, device=rows.device)
-        launch("i8moe_moe_unpermute", rows.device, rows.data_ptr(), _DT[rows.dtype],
-               weights.data_ptr(), inv.data_ptr(), *_eft_args(eft), weights.size(0),
-               weights.size(1), rows.size(1), out.data_ptr())
-        ctx.save_for_backward(rows, weights, inv, eft)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        rows, weights, inv, eft = ctx.saved_tensors
-        dy, dw = moe_unpermute_backward(grad, rows, weights, inv, eft)
-        return (dy if ctx.needs_input_grad[0] else None,
-                dw if ctx.needs_input_grad[1] else None, None, None)
-
-
 def moe_permute_train(hidden_states, topk_ids, n_expert: int, n_local_expert: int = -1,
                       expert_map=None):
     """``moe_permute`` for training: differentiable in hidden_states (once).
@@ -291,37 +158,30 @@ def moe_permute_train(hidden_states, topk_ids, n_expert: int, n_local_expert: in
     Returns (permuted_hidden_states [T * topk, hidden],
     expert_first_token_offset, inv_permuted_idx (flat), permuted_idx); rows of
     no local expert are zero and give no gradient."""
-    what = "moe_permute_train"
-    _check_rows(what, "hidden_states", hidden_states)
-    dev = hidden_states.device
-    _check(topk_ids.dim() == 2 and topk_ids.size(0) == hidden_states.size(0)
-           and topk_ids.size(1) >= 1 and topk_ids.device == dev,
-           f"{what}: topk_ids must have shape [n_token, topk] on hidden_states' device")
-    _check(not topk_ids.is_floating_point(), f"{what}: topk_ids must be integers")
-    if n_local_expert == -1:
-        n_local_expert = n_expert
-    _check(1 <= n_expert <= 2048 and 0 <= n_local_expert <= n_expert,
-           f"{what}: n_expert must be in [1, 2048] and n_local_expert in [0, n_expert]")
-    if expert_map is not None:
-        _check(expert_map.dtype == torch.int32 and expert_map.is_contiguous()
-               and expert_map.device == dev and expert_map.shape == (n_expert,),
-               f"{what}: expert_map must be contiguous int32 [n_expert] on hidden_states' device")
-    ids = topk_ids.to(torch.int32).contiguous()
-    return _SortRows.apply(_aligned(hidden_states), ids, expert_map, n_expert, n_local_expert)
+    return TORCH_OPS.moe_permute_train(hidden_states, topk_ids, n_expert, n_local_expert,
+                                       expert_map)
 
 
 def moe_unpermute_train(permuted_hidden_states, topk_weights, inv_permuted_idx,
                         expert_first_token_offset=None):
     """``moe_unpermute`` for training: returns [n_token, hidden],
-    differentiable in permuted_hidden_states and topk_weights (once)."""
-    what = "moe_unpermute_train"
-    _check_rows(what, "permuted_hidden_states", permuted_hidden_states)
-    dev = permuted_hidden_states.device
-    _check(topk_weights.dim() == 2 and topk_weights.size(1) >= 1 and topk_weights.device == dev
-           and permuted_hidden_states.size(0) == topk_weights.numel(),
-           f"{what}: permuted_hidden_states must have one row per element of topk_weights "
-           "[n_token, topk]")
-    _check_maps(what, inv_permuted_idx, expert_first_token_offset, topk_weights.numel(), dev)
-    return _ReturnRows.apply(_aligned(permuted_hidden_states),
-                             topk_weights.to(torch.float32).contiguous(), inv_permuted_idx,
-                             expert_first_token_offset)
+    differentiable in permuted_hidden_states and topk_weights (once).  Entries
+    of inv_permuted_idx must be rows."""
+    return TORCH_OPS.moe_unpermute_train(permuted_hidden_states, topk_weights, inv_permuted_idx,
+                                         expert_first_token_offset)
+
+
+def moe_permute_backward(permuted_grad, inv_permuted_idx, expert_first_token_offset, n_token: int,
+                         topk: int):
+    """Gradient of the row copy: [n_token, hidden], the sum of each token's
+    rows of ``permuted_grad`` that belong to local experts."""
+    return TORCH_OPS.moe_permute_backward(permuted_grad, inv_permuted_idx,
+                                          expert_first_token_offset, n_token, topk)
+
+
+def moe_unpermute_backward(out_grad, permuted_hidden_states, topk_weights, inv_permuted_idx,
+                           expert_first_token_offset=None):
+    """Gradients of ``moe_unpermute``: (of permuted_hidden_states, of
+    topk_weights in fp32); zero for rows of no local expert."""
+    return TORCH_OPS.moe_unpermute_backward(out_grad, permuted_hidden_states, topk_weights,
+                                            inv_permuted_idx, expert_first_token_offset)
