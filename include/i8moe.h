@@ -212,15 +212,16 @@ int i8moe_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_
 /* Bytes of scratch that i8moe_rms_norm_backward needs when it is given
  * dweight. */
 size_t i8moe_rms_norm_backward_workspace_size(int64_t n_rows, int64_t n_hidden);
-/* Gradients: with n = h * rstd and a = dy * weight,
+/* Gradients: with h = x + residual (residual may be NULL), n = h * rstd and
+ * a = dy * weight,
  *   dx = rstd * (a - n * mean(a * n)) + residual_grad   (x's and residual's)
  *   dweight = sum over rows of dy * n
- * h is residual_out (x without a residual), rstd as i8moe_rms_norm wrote it,
- * residual_grad the gradient of residual_out or NULL; dweight may be NULL.
- * Sums are fp32 in a fixed order. */
+ * rstd as i8moe_rms_norm wrote it, residual_grad the gradient of residual_out
+ * or NULL; dweight may be NULL.  Sums are fp32 in a fixed order. */
 int i8moe_rms_norm_backward(const void* dy, int64_t dy_stride, const void* residual_grad,
-                            int64_t residual_grad_stride, const void* h, int64_t h_stride,
-                            int dtype, const void* weight, int weight_dtype, const float* rstd,
+                            int64_t residual_grad_stride, const void* x, int64_t x_stride,
+                            const void* residual, int64_t residual_stride, int dtype,
+                            const void* weight, int weight_dtype, const float* rstd,
                             int64_t n_rows, int64_t n_hidden, void* dx, void* dweight,
                             void* workspace, size_t workspace_bytes, i8moe_stream_t stream);
 

@@ -57,8 +57,8 @@ PROTOTYPES = {
     "i8moe_moe_unpermute_backward": (I32, [P, P, I32, P, P, P, I64, I64, I64, I64, P, P, P]),
     "i8moe_rms_norm": (I32, [P, I64, P, I64, I32, P, I32, I64, I64, c_float, P, P, P, P, P, P]),
     "i8moe_rms_norm_backward_workspace_size": (c_size_t, [I64, I64]),
-    "i8moe_rms_norm_backward": (I32, [P, I64, P, I64, P, I64, I32, P, I32, P, I64, I64, P, P, P,
-                                      c_size_t, P]),
+    "i8moe_rms_norm_backward": (I32, [P, I64, P, I64, P, I64, P, I64, I32, P, I32, P, I64, I64, P,
+                                      P, P, c_size_t, P]),
     "i8moe_silu_and_mul": (I32, [P, P, I32, I64, I64, P]),
     "i8moe_scale_offsets": (I32, [P, I64, I64, P, P]),
     "i8moe_quant_grouped": (I32, [P, I32, I64, I64, P, I64, I64, I64, I64, I64, P, P, P, P, I32,

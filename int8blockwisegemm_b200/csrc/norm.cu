@@ -11,7 +11,9 @@
 // and, with n = h * rstd and a = dy * weight,
 //   dx = dresidual = rstd * (a - n * mean(a * n)) + dh
 //   dweight = sum over rows of dy * n.
-// Everything between the loads and the stores is fp32.
+// Everything between the loads and the stores is fp32.  The backward pass adds x
+// and the residual again instead of reading the stored h: its rounding would be
+// the larger half of dweight's error.
 #include <algorithm>
 
 #include "common.cuh"
@@ -271,11 +273,12 @@ __global__ void __launch_bounds__(256) norm_wide_kernel(NormArgs a) {
 }
 
 struct NormGradArgs {
-  const void* dy;  // nullable
-  const void* dh;  // nullable
-  const void* h;
+  const void* x;
+  const void* residual;  // nullable
+  const void* dy;
+  const void* dh;  // nullable: the gradient of the residual stream
   const void* weight;
-  int64_t dy_stride, dh_stride, h_stride;
+  int64_t x_stride, residual_stride, dy_stride, dh_stride;
   int weight_dtype;
   const float* rstd;
   int64_t rows;
@@ -286,14 +289,18 @@ struct NormGradArgs {
   int n_part;
 };
 
-constexpr int kGradThreads = 512;
 template <int kPer>
-constexpr int kGradStages = kPer > 2 ? 2 : 3;  // rows of a group in shared memory
-template <int kVec, int kPer>
-constexpr int kGradCtas = kPer <= (kVec == 1 ? 4 : 1) ? 2 : 1;  // resident on an SM
+constexpr int kGradStages = kPer > 2 ? 1 : 3;  // rows of a group in shared memory
+// Threads of a CTA whose groups have that many, and CTAs resident on an SM:
+// 768 threads of 80 registers (1024 of 64 spilled: 52 instead of 36 us), for
+// one group of 512 threads 1024, for more packs a thread 512.
+template <int kThreads>
+constexpr int kGradThreads = kThreads > 256 ? kThreads : 256;
+template <int kVec, int kPer, int kThreads>
+constexpr int kGradCtas = kThreads <= 256 ? 3 : kPer <= (kVec == 1 ? 4 : 1) ? 2 : 1;
 // The most CTAs of a backward pass, and partial sums of the weight's gradient
 // that it writes (one row of k each) before they are added up.
-constexpr int kNormParts = 296;
+constexpr int kNormParts = 444;
 
 // The kThreads threads of a group hold a row's columns, kPer packs each, for
 // all rows that the group takes, and add up their share of the weight's
@@ -305,31 +312,36 @@ constexpr int kNormParts = 296;
 // Single elements (kVec 1) do wait in registers, of which they take few.  A
 // CTA's groups meet at its end.  The grid is what is resident at once.
 template <typename T, int kVec, int kPer, int kThreads, bool kWeight>
-__global__ void __launch_bounds__(kGradThreads, kGradCtas<kVec, kPer>)
+__global__ void __launch_bounds__(kGradThreads<kThreads>, kGradCtas<kVec, kPer, kThreads>)
     norm_grad_row_kernel(NormGradArgs a) {
   using P = Pack<T, kVec>;
+  constexpr int kCta = kGradThreads<kThreads>;
   constexpr bool kRing = kVec > 1;
-  constexpr int kGroups = kGradThreads / kThreads, kWarps = kThreads / 32;
+  constexpr int kGroups = kCta / kThreads, kWarps = kThreads / 32;
   constexpr int kStages = kGradStages<kPer>;
-  extern __shared__ uint4 s_ring[];  // [stage][h, dy, dh][kPer][thread of the CTA]
-  __shared__ float s_part[2][kGradThreads / 32];
+  extern __shared__ uint4 s_ring[];  // [stage][x, dy, residual, dh][kPer][thread of the CTA]
+  __shared__ float s_part[2][kCta / 32];
   const int group = threadIdx.x / kThreads, tid = threadIdx.x % kThreads;
   const int lane = tid & 31;
   const int64_t rows_at_once = static_cast<int64_t>(gridDim.x) * kGroups;
   int64_t r = static_cast<int64_t>(group) * gridDim.x + blockIdx.x;
   auto row_of = [&](int which, int64_t row) {
-    return which == 0   ? static_cast<const T*>(a.h) + row * a.h_stride
+    return which == 0   ? static_cast<const T*>(a.x) + row * a.x_stride
            : which == 1 ? static_cast<const T*>(a.dy) + row * a.dy_stride
+           : which == 2 ? static_cast<const T*>(a.residual) + row * a.residual_stride
                         : static_cast<const T*>(a.dh) + row * a.dh_stride;
   };
+  auto there = [&](int which) {
+    return which < 2 || (which == 2 ? a.residual : a.dh) != nullptr;
+  };
   auto ring = [&](int stage, int which, int p) {
-    return s_ring + ((stage * 3 + which) * kPer + p) * kGradThreads + threadIdx.x;
+    return s_ring + ((stage * 4 + which) * kPer + p) * kCta + threadIdx.x;
   };
   auto copy = [&](int64_t row, int stage) {
     if (row < a.rows)
 #pragma unroll
-      for (int which = 0; which < 3; ++which)
-        if (which < 2 || a.dh)
+      for (int which = 0; which < 4; ++which)
+        if (there(which))
 #pragma unroll
           for (int p = 0; p < kPer; ++p) {
             const int i = (p * kThreads + tid) * kVec;
@@ -341,14 +353,14 @@ __global__ void __launch_bounds__(kGradThreads, kGradCtas<kVec, kPer>)
           }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  P now[kRing ? 1 : 3][kPer], next[kRing ? 1 : 3][kPer];
+  P now[kRing ? 1 : 4][kPer], next[kRing ? 1 : 4][kPer];
   auto load = [&](int64_t row) {
 #pragma unroll
-    for (int which = 0; which < 3; ++which)
+    for (int which = 0; which < 4; ++which)
 #pragma unroll
       for (int p = 0; p < kPer; ++p) {
         const int i = (p * kThreads + tid) * kVec;
-        if (i < a.k && (which < 2 || a.dh))
+        if (i < a.k && there(which))
           next[kRing ? 0 : which][p] = *reinterpret_cast<const P*>(row_of(which, row) + i);
       }
   };
@@ -379,7 +391,7 @@ __global__ void __launch_bounds__(kGradThreads, kGradCtas<kVec, kPer>)
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     } else {
 #pragma unroll
-      for (int which = 0; which < 3; ++which)
+      for (int which = 0; which < 4; ++which)
 #pragma unroll
         for (int p = 0; p < kPer; ++p) now[which][p] = next[which][p];
       if (r + rows_at_once < a.rows) load(r + rows_at_once);
@@ -389,10 +401,14 @@ __global__ void __launch_bounds__(kGradThreads, kGradCtas<kVec, kPer>)
     for (int p = 0; p < kPer; ++p) {
       const int i = (p * kThreads + tid) * kVec;
       if (i < a.k) {
-        const P h = get(stage, 0, p), g = get(stage, 1, p);
+        const P x = get(stage, 0, p), g = get(stage, 1, p);
+        P res;
+        if (a.residual) res = get(stage, 2, p);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          const float hf = Num<T>::to_f(h.v[e]), gf = Num<T>::to_f(g.v[e]);
+          float hf = Num<T>::to_f(x.v[e]);
+          if (a.residual) hf += Num<T>::to_f(res.v[e]);
+          const float gf = Num<T>::to_f(g.v[e]);
           if constexpr (kWeight) dw[p][e] = fmaf(gf * rstd, hf, dw[p][e]);
           dot = fmaf(gf * w[p][e], hf, dot);
         }
@@ -414,12 +430,15 @@ __global__ void __launch_bounds__(kGradThreads, kGradCtas<kVec, kPer>)
     for (int p = 0; p < kPer; ++p) {
       const int i = (p * kThreads + tid) * kVec;
       if (i < a.k) {
-        const P h = get(stage, 0, p), g = get(stage, 1, p);
-        P o, add;
-        if (a.dh) add = get(stage, 2, p);
+        const P x = get(stage, 0, p), g = get(stage, 1, p);
+        P o, res, add;
+        if (a.residual) res = get(stage, 2, p);
+        if (a.dh) add = get(stage, 3, p);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          float d = Num<T>::to_f(h.v[e]) * back;
+          float d = Num<T>::to_f(x.v[e]);
+          if (a.residual) d += Num<T>::to_f(res.v[e]);
+          d *= back;
           d = fmaf(Num<T>::to_f(g.v[e]) * w[p][e], rstd, d);
           if (a.dh) d += Num<T>::to_f(add.v[e]);
           o.v[e] = Num<T>::from_f(d);
@@ -462,25 +481,37 @@ __global__ void __launch_bounds__(kGradThreads, kGradCtas<kVec, kPer>)
   }
 }
 
+// h of one row, element by element
+template <typename T>
+struct SumRow {
+  const T* x;
+  const T* residual;
+  __device__ __forceinline__ SumRow(const NormGradArgs& a, int64_t r)
+      : x(static_cast<const T*>(a.x) + r * a.x_stride),
+        residual(a.residual ? static_cast<const T*>(a.residual) + r * a.residual_stride : nullptr) {}
+  __device__ __forceinline__ float operator[](int i) const {
+    const float v = Num<T>::to_f(x[i]);
+    return residual ? v + Num<T>::to_f(residual[i]) : v;
+  }
+};
+
 // Rows too wide for the registers of a CTA: read twice, and once more for the
 // weight's gradient.
 template <typename T>
 __global__ void __launch_bounds__(256) norm_grad_wide_kernel(NormGradArgs a) {
   __shared__ float s_part[8];
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const T* h = static_cast<const T*>(a.h) + r * a.h_stride;
+    const SumRow<T> h(a, r);
     const T* dy = static_cast<const T*>(a.dy) + r * a.dy_stride;
     const T* dh = a.dh ? static_cast<const T*>(a.dh) + r * a.dh_stride : nullptr;
     const float rstd = a.rstd[r];
     float dot = 0.f;
     for (int i = threadIdx.x; i < a.k; i += blockDim.x)
-      dot += Num<T>::to_f(dy[i]) * load_any(a.weight, a.weight_dtype, i) *
-             (Num<T>::to_f(h[i]) * rstd);
+      dot += Num<T>::to_f(dy[i]) * load_any(a.weight, a.weight_dtype, i) * (h[i] * rstd);
     const float mean = block_reduce<Sum>(dot, s_part) * a.inv_k;
     for (int i = threadIdx.x; i < a.k; i += blockDim.x) {
-      const float n = Num<T>::to_f(h[i]) * rstd;
       const float g = Num<T>::to_f(dy[i]) * load_any(a.weight, a.weight_dtype, i);
-      float d = rstd * (g - n * mean);
+      float d = rstd * (g - h[i] * rstd * mean);
       if (dh) d += Num<T>::to_f(dh[i]);
       static_cast<T*>(a.dx)[r * a.k + i] = Num<T>::from_f(d);
     }
@@ -495,7 +526,7 @@ __global__ void __launch_bounds__(256) norm_weight_part_kernel(NormGradArgs a) {
   float s = 0.f;
   for (int64_t r = blockIdx.y; r < a.rows; r += a.n_part)
     s = fmaf(Num<T>::to_f(static_cast<const T*>(a.dy)[r * a.dy_stride + i]),
-             Num<T>::to_f(static_cast<const T*>(a.h)[r * a.h_stride + i]) * a.rstd[r], s);
+             SumRow<T>(a, r)[i] * a.rstd[r], s);
   a.part[static_cast<int64_t>(blockIdx.y) * a.k + i] = s;
 }
 
@@ -562,18 +593,18 @@ int launch_norm(const NormArgs& a, cudaStream_t st) {
 
 template <typename T, int kVec, int kPer, int kThreads>
 int launch_norm_grad_kernel(NormGradArgs& a, cudaStream_t st) {
-  const int64_t groups = kGradThreads / kThreads;
-  const int64_t most = int64_t(num_sms(current_device())) * kGradCtas<kVec, kPer>;
+  constexpr int kCta = kGradThreads<kThreads>, kGroups = kCta / kThreads;
+  const int64_t most = int64_t(num_sms(current_device())) * kGradCtas<kVec, kPer, kThreads>;
   a.n_part = static_cast<int>(
-      std::min({(a.rows + groups - 1) / groups, most, int64_t(kNormParts)}));
-  constexpr int kRing = kVec > 1 ? kGradStages<kPer> * 3 * kPer * kGradThreads * 16 : 0;
-  constexpr int kMeet = (kGradThreads / kThreads - 1) * kPer * kVec * kThreads * 4;
+      std::min({(a.rows + kGroups - 1) / kGroups, most, int64_t(kNormParts)}));
+  constexpr int kRing = kVec > 1 ? kGradStages<kPer> * 4 * kPer * kCta * 16 : 0;
+  constexpr int kMeet = (kGroups - 1) * kPer * kVec * kThreads * 4;
   constexpr int kSmem = kRing > kMeet ? kRing : kMeet;
   auto kernel = a.part ? norm_grad_row_kernel<T, kVec, kPer, kThreads, true>
                        : norm_grad_row_kernel<T, kVec, kPer, kThreads, false>;
-  if (kSmem > 48 * 1024)
+  if (kSmem > 40 * 1024)  // with the static part, more than every kernel may have
     I8_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-  kernel<<<a.n_part, kGradThreads, kSmem, st>>>(a);
+  kernel<<<a.n_part, kCta, kSmem, st>>>(a);
   return check_launch("rms_norm_backward");
 }
 
@@ -596,9 +627,11 @@ int launch_norm_grad_rows(NormGradArgs& a, cudaStream_t st, bool* wide) {
 template <typename T>
 int launch_norm_grad(NormGradArgs& a, cudaStream_t st) {
   constexpr int kVec = 16 / sizeof(T);
-  const bool packs = a.k % kVec == 0 && a.h_stride % kVec == 0 && a.dy_stride % kVec == 0 &&
+  const bool packs = a.k % kVec == 0 && a.x_stride % kVec == 0 && a.dy_stride % kVec == 0 &&
+                     (!a.residual || a.residual_stride % kVec == 0) &&
                      (!a.dh || a.dh_stride % kVec == 0) &&
-                     (bits(a.h) | bits(a.dy) | bits(a.dh) | bits(a.weight) | bits(a.dx)) % 16 == 0;
+                     (bits(a.x) | bits(a.residual) | bits(a.dy) | bits(a.dh) | bits(a.weight) |
+                      bits(a.dx)) % 16 == 0;
   bool wide = false;
   const int rc = packs ? launch_norm_grad_rows<T, kVec>(a, st, &wide)
                        : launch_norm_grad_rows<T, 1>(a, st, &wide);
@@ -649,8 +682,9 @@ size_t i8moe_rms_norm_backward_workspace_size(int64_t n_rows, int64_t n_hidden) 
 }
 
 int i8moe_rms_norm_backward(const void* dy, int64_t dy_stride, const void* residual_grad,
-                            int64_t residual_grad_stride, const void* h, int64_t h_stride,
-                            int dtype, const void* weight, int weight_dtype, const float* rstd,
+                            int64_t residual_grad_stride, const void* x, int64_t x_stride,
+                            const void* residual, int64_t residual_stride, int dtype,
+                            const void* weight, int weight_dtype, const float* rstd,
                             int64_t n_rows, int64_t n_hidden, void* dx, void* dweight,
                             void* workspace, size_t workspace_bytes, i8moe_stream_t stream) {
   I8_REQUIRE(float_dtype(dtype), "rms_norm_backward: unsupported dtype");
@@ -664,10 +698,10 @@ int i8moe_rms_norm_backward(const void* dy, int64_t dy_stride, const void* resid
       I8_CUDA(cudaMemsetAsync(dweight, 0, n_hidden * (weight_dtype == I8MOE_FP32 ? 4 : 2), st));
     return I8MOE_OK;
   }
-  I8_REQUIRE(dy && h && weight && rstd && dx,
-             "rms_norm_backward: dy, h, weight, rstd and dx must be given");
-  NormGradArgs a{dy, residual_grad, h, weight, dy_stride, residual_grad_stride, h_stride,
-                 weight_dtype, rstd, n_rows, static_cast<int>(n_hidden),
+  I8_REQUIRE(dy && x && weight && rstd && dx,
+             "rms_norm_backward: dy, x, weight, rstd and dx must be given");
+  NormGradArgs a{x, residual, dy, residual_grad, weight, x_stride, residual_stride, dy_stride,
+                 residual_grad_stride, weight_dtype, rstd, n_rows, static_cast<int>(n_hidden),
                  1.f / static_cast<float>(n_hidden), dx, nullptr, 0};
   if (dweight) {
     I8_REQUIRE(workspace != nullptr && workspace_bytes >= i8moe_rms_norm_backward_workspace_size(

@@ -130,40 +130,46 @@ Tensor norm_forward(const Tensor& x, const Tensor& weight, double eps,
   return h;
 }
 
-std::tuple<Tensor, optional<Tensor>> rms_norm_backward(const Tensor& dy, const Tensor& h,
-                                                       const Tensor& weight, const Tensor& rstd,
-                                                       const optional<Tensor>& residual_grad,
-                                                       bool weight_grad) {
+std::tuple<Tensor, optional<Tensor>> rms_norm_backward(
+    const Tensor& dy, const Tensor& x, const Tensor& weight, const Tensor& rstd,
+    const optional<Tensor>& residual, const optional<Tensor>& residual_grad, bool weight_grad) {
   const char* what = "rms_norm_backward";
-  check_norm(what, h, weight, 0.0, residual_grad);
-  TORCH_CHECK(dy.sizes() == h.sizes() && dy.scalar_type() == h.scalar_type() &&
-                  dy.device() == h.device(),
-              what, ": dy must have h's shape, dtype and device");
+  check_norm(what, x, weight, 0.0, residual);
+  auto like_x = [&](const Tensor& t) {
+    return t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device();
+  };
+  TORCH_CHECK(like_x(dy), what, ": dy must have x's shape, dtype and device");
+  TORCH_CHECK(!residual_grad || like_x(*residual_grad), what,
+              ": residual_grad must have x's shape, dtype and device");
   TORCH_CHECK(rstd.scalar_type() == at::kFloat && rstd.is_contiguous() &&
-                  rstd.device() == h.device() && rstd.numel() == h.numel() / h.size(-1),
-              what, ": rstd must be float32 [rows] on h's device");
-  const c10::cuda::CUDAGuard guard(h.device());
-  const Tensor hr = rows_of(h), gr = rows_of(dy), w = weight.contiguous();
-  Tensor rr;
-  if (residual_grad) rr = rows_of(*residual_grad);
-  Tensor dx = empty(h.sizes(), h, h.scalar_type());
+                  rstd.device() == x.device() && rstd.numel() == x.numel() / x.size(-1),
+              what, ": rstd must be float32 [rows] on x's device");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor xr = rows_of(x), gr = rows_of(dy), w = weight.contiguous();
+  Tensor rr, hr;
+  if (residual) rr = rows_of(*residual);
+  if (residual_grad) hr = rows_of(*residual_grad);
+  Tensor dx = empty(x.sizes(), x, x.scalar_type());
   optional<Tensor> dw;
   Tensor workspace;
   size_t bytes = 0;
   if (weight_grad) {
-    dw = empty(weight.sizes(), h, weight.scalar_type());
-    bytes = lib.rms_norm_backward_workspace_size(hr.size(0), hr.size(1));
-    workspace = empty({static_cast<int64_t>(bytes)}, h, at::kByte);
+    dw = empty(weight.sizes(), x, weight.scalar_type());
+    bytes = lib.rms_norm_backward_workspace_size(xr.size(0), xr.size(1));
+    workspace = empty({static_cast<int64_t>(bytes)}, x, at::kByte);
   }
-  check(lib.rms_norm_backward(gr.data_ptr(), gr.stride(0), residual_grad ? rr.data_ptr() : nullptr,
-                              residual_grad ? rr.stride(0) : 0, hr.data_ptr(), hr.stride(0),
-                              type_of(h), w.data_ptr(), type_of(w),
-                              static_cast<const float*>(rstd.data_ptr()), hr.size(0), hr.size(1),
+  check(lib.rms_norm_backward(gr.data_ptr(), gr.stride(0), residual_grad ? hr.data_ptr() : nullptr,
+                              residual_grad ? hr.stride(0) : 0, xr.data_ptr(), xr.stride(0),
+                              residual ? rr.data_ptr() : nullptr, residual ? rr.stride(0) : 0,
+                              type_of(x), w.data_ptr(), type_of(w),
+                              static_cast<const float*>(rstd.data_ptr()), xr.size(0), xr.size(1),
                               dx.data_ptr(), dw ? dw->data_ptr() : nullptr,
-                              dw ? workspace.data_ptr() : nullptr, bytes, stream_of(h)),
+                              dw ? workspace.data_ptr() : nullptr, bytes, stream_of(x)),
         what);
   return {dx, dw};
 }
+
+optional<Tensor> some(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
 
 struct RmsNorm : torch::autograd::Function<RmsNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
@@ -171,7 +177,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     Tensor y = empty(x.sizes(), x, x.scalar_type());
     Tensor rstd = empty({x.numel() / x.size(-1)}, x, at::kFloat);
     const Tensor h = norm_forward(x, weight, eps, residual, &y, &rstd, nullptr, nullptr);
-    ctx->save_for_backward({residual ? h : x, weight, rstd});
+    ctx->save_for_backward({x, weight, rstd, residual ? *residual : Tensor()});
     ctx->set_materialize_grads(false);
     return residual ? variable_list{y, h} : variable_list{y};
   }
@@ -184,8 +190,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
       return {dh, Tensor(), Tensor(), two ? dh : Tensor()};
     const variable_list saved = ctx->get_saved_variables();
     const auto [dx, dw] =
-        rms_norm_backward(grads[0], saved[0], saved[1], saved[2],
-                          dh.defined() ? optional<Tensor>(dh) : std::nullopt,
+        rms_norm_backward(grads[0], saved[0], saved[1], saved[2], some(saved[3]), some(dh),
                           ctx->needs_input_grad(1));
     return {dx, dw ? *dw : Tensor(), Tensor(), two ? dx : Tensor()};
   }
@@ -360,9 +365,8 @@ struct ReturnRows : torch::autograd::Function<ReturnRows> {
     once("moe_unpermute_train");
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     const variable_list saved = ctx->get_saved_variables();
-    const auto [dy, dw] = moe_unpermute_backward(
-        grads[0], saved[0], saved[1], saved[2],
-        saved[3].defined() ? optional<Tensor>(saved[3]) : std::nullopt);
+    const auto [dy, dw] =
+        moe_unpermute_backward(grads[0], saved[0], saved[1], saved[2], some(saved[3]));
     return {ctx->needs_input_grad(0) ? dy : Tensor(), ctx->needs_input_grad(1) ? dw : Tensor(),
             Tensor(), Tensor()};
   }

@@ -8,7 +8,8 @@ reference counterpart), differentiable, and with an int8 output.
 type.  ``rms_norm_quant_int8`` gives y as int8 with one scale per token, the
 ``a`` / ``a_row_scale`` of ``ops.int8_grouped_mm_scaled``, and on request y as
 well, for the router.  Sums, norms and scales are fp32; y and the int8 values
-come from the unrounded h.
+come from the unrounded h, and so do the gradients (x and residual are kept for
+them).
 
 x is [..., K] in bf16, fp16 or fp32 on a CUDA device, of any K and alignment;
 rows may have any stride (a last dimension that is not contiguous is copied).
@@ -39,8 +40,9 @@ def rms_norm_quant_int8(x, weight, eps: float = 1e-6, residual=None, return_norm
     return TORCH_OPS.rms_norm_quant_int8(x, weight, eps, residual, return_norm)
 
 
-def rms_norm_backward(dy, h, weight, rstd, residual_grad=None, weight_grad: bool = True):
+def rms_norm_backward(dy, x, weight, rstd, residual=None, residual_grad=None,
+                      weight_grad: bool = True):
     """Gradients of ``rms_norm``: (gradient of x and residual, gradient of
-    weight or None).  ``h`` is the residual stream (x without a residual),
-    ``rstd`` fp32 [rows] = 1 / sqrt(mean(h^2) + eps)."""
-    return TORCH_OPS.rms_norm_backward(dy, h, weight, rstd, residual_grad, weight_grad)
+    weight or None).  ``rstd`` is fp32 [rows] = 1 / sqrt(mean(h^2) + eps) of
+    h = x + residual, ``residual_grad`` the gradient of h as an output."""
+    return TORCH_OPS.rms_norm_backward(dy, x, weight, rstd, residual, residual_grad, weight_grad)

@@ -135,9 +135,7 @@ def check_grad(x, w, r, eps, dy, dh):
     out = norm.rms_norm(leaves[0], leaves[1], eps, leaves[2] if r is not None else None)
     outs, grads = ([out], [dy]) if r is None else (list(out), [dy, dh])
     got = torch.autograd.grad(outs, leaves, grads)
-    # the formula at the stored residual stream
-    h = (x if r is None else out[1].detach()).double()
-    _, rstd, _ = formula(x, w, r, eps)
+    h, rstd, _ = formula(x, w, r, eps)
     n, a = h * rstd, dy.double() * w.double()
     mean = (a * n).mean(-1, keepdim=True)
     dx = rstd * (a - n * mean)
@@ -219,8 +217,11 @@ def test_partial_gradients_and_unused_outputs():
     assert x.grad.shape == (0, 64) and not w.grad.any()
     with torch.no_grad():
         assert not norm.rms_norm(x, w).requires_grad
-    y, h = norm.rms_norm(r, w, 1e-6, r)
-    h.add_(1)  # the residual stream is kept for the backward pass
+    z = r.detach().clone()
+    y, h = norm.rms_norm(r, w, 1e-6, z)
+    h.add_(1)  # the next block may go on in place
+    y.sum().backward(retain_graph=True)
+    z.add_(1)  # what the backward pass needs may not change
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
 
@@ -281,10 +282,14 @@ def test_refusals():
                 f(**args)
     with pytest.raises(RuntimeError, match="no gradient"):
         norm.rms_norm_quant_int8(x, w.clone().requires_grad_())
-    with pytest.raises(RuntimeError, match="h's shape"):
+    with pytest.raises(RuntimeError, match="x's shape"):
         norm.rms_norm_backward(x[:2], x, w, torch.ones(4, device=DEV))
     with pytest.raises(RuntimeError, match="rstd"):
         norm.rms_norm_backward(x, x, w, torch.ones(3, device=DEV))
+    one = torch.ones(4, device=DEV)
+    for args, message in [((x, x, w, one, r[:2]), "residual must"), ((x, x, w, one, r, r.float()), "residual_grad")]:
+        with pytest.raises(RuntimeError, match=message):
+            norm.rms_norm_backward(*args)
 
 
 def test_refuses_cpu_tensors():
@@ -314,8 +319,8 @@ def test_c_argument_errors_before_any_cuda_call():
     assert big == lib.i8moe_rms_norm_backward_workspace_size(1 << 30, 2048)
 
     def backward(dtype=0, wdtype=0, rows=4, k=8, dy=one, dw=None, ws=None, nbytes=0):
-        return lib.i8moe_rms_norm_backward(dy, k, None, 0, one, k, dtype, one, wdtype, one, rows, k, one, dw, ws,
-                                           nbytes, None)
+        return lib.i8moe_rms_norm_backward(dy, k, None, 0, one, k, None, 0, dtype, one, wdtype, one, rows, k, one, dw,
+                                           ws, nbytes, None)
 
     for kw, message in [(dict(dtype=5, wdtype=5), "dtype"), (dict(wdtype=1), "weight"), (dict(rows=-1), "n_rows"),
                         (dict(k=0), "n_hidden"), (dict(dy=None), "must be given"), (dict(dw=one), "workspace"),
