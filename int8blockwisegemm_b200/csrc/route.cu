@@ -414,80 +414,21 @@ __global__ void expand_rows(const uint4* __restrict__ in, uint4* __restrict__ ou
 }
 
 // out[t] = dtype(sum_j fma(w[t,j], x[inv[t,j]], acc)), fp32 accumulation in
-// j order (finalizeMoeRoutingKernel, .inl:132-188).  Two tokens per CTA:
-// both tokens' inverse indices, then all their rows, are in flight together
-// (one token per CTA measured 66.8 against 63.5 us at the default shape).
+// j order (finalizeMoeRoutingKernel, .inl:132-188).  One token per CTA, four of
+// its rows in flight: loads without a condition (rows that do not count are
+// replaced by the first one, whose values are dropped), so that the compiler
+// issues them together.
 template <typename T>
-__global__ void __launch_bounds__(256) unpermute_kernel(const T* __restrict__ x,
-                                                        const float* __restrict__ w,
-                                                        const int32_t* __restrict__ inv,
-                                                        const int64_t* eft, int n_local, int topk,
-                                                        int vecs_per_row, T* __restrict__ out,
-                                                        int n_token) {
+__global__ void __launch_bounds__(256, 6) unpermute_kernel(const T* __restrict__ x,
+                                                           const float* __restrict__ w,
+                                                           const int32_t* __restrict__ inv,
+                                                           const int64_t* eft, int n_local,
+                                                           int topk, int vecs_per_row,
+                                                           T* __restrict__ out) {
   constexpr int EPV = 16 / sizeof(T);
-  constexpr int G = 8;    // source rows in flight per token
-  constexpr int TPC = 2;  // tokens per CTA
-  const int t0 = blockIdx.x * TPC;
+  constexpr int G = 4;  // source rows in flight
+  const int64_t t = blockIdx.x;
   const int64_t valid = eft ? eft[n_local] : INT64_MAX;
-  for (int v = threadIdx.x; v < vecs_per_row; v += blockDim.x) {
-    float acc[TPC][EPV];
-#pragma unroll
-    for (int tt = 0; tt < TPC; ++tt)
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) acc[tt][e] = 0.f;
-    for (int j0 = 0; j0 < topk; j0 += G) {
-      uint4 raw[TPC][G];
-      int idx[TPC][G];
-#pragma unroll
-      for (int tt = 0; tt < TPC; ++tt)
-#pragma unroll
-        for (int j = 0; j < G; ++j)
-          idx[tt][j] = (t0 + tt < n_token && j0 + j < topk)
-                           ? __ldg(inv + static_cast<int64_t>(t0 + tt) * topk + j0 + j)
-                           : -1;
-#pragma unroll
-      for (int tt = 0; tt < TPC; ++tt)
-#pragma unroll
-        for (int j = 0; j < G; ++j)
-          if (idx[tt][j] >= 0 && idx[tt][j] < valid)
-            raw[tt][j] = __ldg(reinterpret_cast<const uint4*>(x) +
-                               static_cast<int64_t>(idx[tt][j]) * vecs_per_row + v);
-#pragma unroll
-      for (int tt = 0; tt < TPC; ++tt)
-#pragma unroll
-        for (int j = 0; j < G; ++j) {
-          if (idx[tt][j] >= 0 && idx[tt][j] < valid) {
-            const float wt = __ldg(w + static_cast<int64_t>(t0 + tt) * topk + j0 + j);
-            const T* e8 = reinterpret_cast<const T*>(&raw[tt][j]);
-#pragma unroll
-            for (int e = 0; e < EPV; ++e) acc[tt][e] = fmaf(wt, Num<T>::to_f(e8[e]), acc[tt][e]);
-          }
-        }
-    }
-#pragma unroll
-    for (int tt = 0; tt < TPC; ++tt) {
-      if (t0 + tt >= n_token) break;
-      uint4 o;
-      T* ov = reinterpret_cast<T*>(&o);
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) ov[e] = Num<T>::from_f(acc[tt][e]);
-      reinterpret_cast<uint4*>(out)[static_cast<int64_t>(t0 + tt) * vecs_per_row + v] = o;
-    }
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) unpermute_kernel(const T* __restrict__ x,
-                                                        const float* __restrict__ w,
-                                                        const int32_t* __restrict__ inv,
-                                                        const int64_t* eft, int n_local, int topk,
-                                                        int vecs_per_row, T* __restrict__ out) {
-  constexpr int EPV = 16 / sizeof(T);
-  constexpr int G = 8;  // source rows in flight per thread
-  const int t = blockIdx.x;
-  const int64_t valid = eft ? eft[n_local] : INT64_MAX;
-  const int32_t* inv_t = inv + static_cast<int64_t>(t) * topk;
-  const float* w_t = w + static_cast<int64_t>(t) * topk;
   for (int v = threadIdx.x; v < vecs_per_row; v += blockDim.x) {
     float acc[EPV];
 #pragma unroll
@@ -495,28 +436,32 @@ __global__ void __launch_bounds__(256) unpermute_kernel(const T* __restrict__ x,
     for (int j0 = 0; j0 < topk; j0 += G) {
       uint4 raw[G];
       int idx[G];
+      float wt[G];
 #pragma unroll
       for (int j = 0; j < G; ++j) {
-        idx[j] = (j0 + j < topk) ? __ldg(inv_t + j0 + j) : -1;
-        if (idx[j] >= 0 && idx[j] < valid)
-          raw[j] = __ldg(reinterpret_cast<const uint4*>(x) +
-                         static_cast<int64_t>(idx[j]) * vecs_per_row + v);
+        const bool in = j0 + j < topk;
+        idx[j] = in ? __ldg(inv + t * topk + j0 + j) : -1;
+        wt[j] = in ? __ldg(w + t * topk + j0 + j) : 0.f;
       }
 #pragma unroll
       for (int j = 0; j < G; ++j) {
-        if (idx[j] >= 0 && idx[j] < valid) {
-          const float wt = __ldg(w_t + j0 + j);
-          const T* e8 = reinterpret_cast<const T*>(&raw[j]);
+        if (idx[j] >= valid) idx[j] = -1;
+        raw[j] = __ldg(reinterpret_cast<const uint4*>(x) +
+                       static_cast<int64_t>(max(idx[j], 0)) * vecs_per_row + v);
+      }
 #pragma unroll
-          for (int e = 0; e < EPV; ++e) acc[e] = fmaf(wt, Num<T>::to_f(e8[e]), acc[e]);
-        }
+      for (int j = 0; j < G; ++j) {
+        const T* e8 = reinterpret_cast<const T*>(&raw[j]);
+#pragma unroll
+        for (int e = 0; e < EPV; ++e)
+          acc[e] = idx[j] < 0 ? acc[e] : fmaf(wt[j], Num<T>::to_f(e8[e]), acc[e]);
       }
     }
     uint4 o;
     T* ov = reinterpret_cast<T*>(&o);
 #pragma unroll
     for (int e = 0; e < EPV; ++e) ov[e] = Num<T>::from_f(acc[e]);
-    reinterpret_cast<uint4*>(out)[static_cast<int64_t>(t) * vecs_per_row + v] = o;
+    reinterpret_cast<uint4*>(out)[t * vecs_per_row + v] = o;
   }
 }
 
@@ -869,19 +814,19 @@ int i8moe_moe_unpermute(const void* permuted_hidden, int dtype, const float* top
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int nl = static_cast<int>(n_local_expert);
   const int k = static_cast<int>(topk);
-  const dim3 grid(static_cast<unsigned>((n_token + 1) / 2));
+  const dim3 grid(static_cast<unsigned>(n_token));
   if (dtype == I8MOE_BF16) {
     unpermute_kernel<__nv_bfloat16><<<grid, threads, 0, st>>>(
         static_cast<const __nv_bfloat16*>(permuted_hidden), topk_weights, inv_permuted_idx,
-        expert_first_token_offset, nl, k, vpr, static_cast<__nv_bfloat16*>(out), static_cast<int>(n_token));
+        expert_first_token_offset, nl, k, vpr, static_cast<__nv_bfloat16*>(out));
   } else if (dtype == I8MOE_FP16) {
     unpermute_kernel<__half><<<grid, threads, 0, st>>>(
         static_cast<const __half*>(permuted_hidden), topk_weights, inv_permuted_idx,
-        expert_first_token_offset, nl, k, vpr, static_cast<__half*>(out), static_cast<int>(n_token));
+        expert_first_token_offset, nl, k, vpr, static_cast<__half*>(out));
   } else {
     unpermute_kernel<float><<<grid, threads, 0, st>>>(
         static_cast<const float*>(permuted_hidden), topk_weights, inv_permuted_idx,
-        expert_first_token_offset, nl, k, vpr, static_cast<float*>(out), static_cast<int>(n_token));
+        expert_first_token_offset, nl, k, vpr, static_cast<float*>(out));
   }
   return check_launch("moe_unpermute");
 }

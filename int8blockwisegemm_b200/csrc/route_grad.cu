@@ -87,11 +87,16 @@ __global__ void __launch_bounds__(256) scatter_rows_kernel(RowArgs a, const uint
   }
 }
 
-// One token per CTA, kSlots of its rows in flight.
+// One token per CTA, four of its rows in flight: loads without a condition
+// (rows that do not count are replaced by the first one, whose values are
+// dropped), so that the compiler issues them together.  Bound by memory: 8192 x
+// 2048 bf16, top 8 (302 MB) takes 47.5 us, 6.4 of the 6.6 TB/s of a copy; with
+// conditional loads 63, with eight rows and registers for four CTAs an SM 56.
 template <typename T>
-__global__ void __launch_bounds__(256) gather_sum_kernel(RowArgs a, const uint4* __restrict__ rows,
-                                                         uint4* __restrict__ out) {
-  constexpr int EPV = 16 / sizeof(T), kSlots = 8;
+__global__ void __launch_bounds__(256, 6) gather_sum_kernel(RowArgs a,
+                                                            const uint4* __restrict__ rows,
+                                                            uint4* __restrict__ out) {
+  constexpr int EPV = 16 / sizeof(T), kSlots = 4;
   const int valid = valid_rows(a);
   const int64_t t = blockIdx.x;
   for (int v = threadIdx.x; v < a.vpr; v += blockDim.x) {
@@ -103,13 +108,15 @@ __global__ void __launch_bounds__(256) gather_sum_kernel(RowArgs a, const uint4*
       uint4 raw[kSlots];
       sorted_rows<kSlots>(a, t, j0, d);
 #pragma unroll
-      for (int j = 0; j < kSlots; ++j)
-        raw[j] = d[j] >= 0 && d[j] < valid ? __ldg(vec(rows, a, d[j], v)) : make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < kSlots; ++j) {
+        if (d[j] >= valid) d[j] = -1;
+        raw[j] = __ldg(vec(rows, a, d[j] < 0 ? 0 : d[j], v));
+      }
 #pragma unroll
       for (int j = 0; j < kSlots; ++j) {
         const T* p = reinterpret_cast<const T*>(&raw[j]);
 #pragma unroll
-        for (int e = 0; e < EPV; ++e) acc[e] += Num<T>::to_f(p[e]);
+        for (int e = 0; e < EPV; ++e) acc[e] += d[j] < 0 ? 0.f : Num<T>::to_f(p[e]);
       }
     }
     uint4 o;
