@@ -4,7 +4,8 @@
 // Routing replaces the reference's CUB radix sort + binary-search offsets +
 // permutation-map kernels (csrc/permute_unpermute_kernels/
 // moe_permute_unpermute_kernel.cu:25-169, .inl:3-118) by three small
-// kernels over chunks of 2048 keys:
+// kernels over chunks of 2048 keys (one kernel does all three steps of a single
+// chunk):
 //   route_hist    -- per-chunk bucket histogram (bucket = key's low
 //                    experts_to_bits(n_expert) bits, the bits CUB sorts on)
 //   route_scan    -- one CTA: per-bucket exclusive scan across chunks and
@@ -220,13 +221,68 @@ __global__ void __launch_bounds__(kThreads) router_kernel(RouterArgs r, RouteArg
   for (int b = threadIdx.x; b < a.nb; b += kThreads) out[b] = s_hist[b];
 }
 
-// Single CTA of 1024 threads.
-__global__ void __launch_bounds__(1024) route_scan(RouteArgs a) {
+// Stable scatter of `rounds` x kThreads keys from key0 on, by the first kThreads
+// threads of a CTA (the others take part in the barriers): `running` holds each
+// bucket's next destination, wcnt [8][nb] zeros.
+__device__ __forceinline__ void scatter_keys(const RouteArgs& a, int key0, int rounds,
+                                             int* running, int* wcnt, int limit) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const unsigned lt_mask = (1u << lane) - 1u;
+  for (int j = 0; j < rounds; ++j) {
+    const int i = key0 + j * kThreads + tid;
+    const bool valid = tid < kThreads && i < a.R;
+    const int b = valid ? route_key(a, i) : a.nb;  // invalid lanes form their own group
+    const unsigned m = __match_any_sync(0xffffffffu, b);
+    const int rank = __popc(m & lt_mask);
+    const int cnt = __popc(m);
+    const bool leader = (m & lt_mask) == 0;
+    if (valid && leader) wcnt[warp * a.nb + b] = cnt;
+    __syncthreads();
+    int dest = 0;
+    if (valid) {
+      dest = running[b] + rank;
+      for (int w = 0; w < warp; ++w) dest += wcnt[w * a.nb + b];
+    }
+    __syncthreads();
+    if (valid && leader) {
+      atomicAdd(&running[b], cnt);
+      wcnt[warp * a.nb + b] = 0;
+    }
+    if (valid) {
+      // token_expert_indices is arange in the reference; null means exactly that
+      const int value = a.values != nullptr ? __ldg(a.values + i) : i;
+      if (value >= 0 && value < a.R) {
+        a.inv[value] = dest;
+      } else {
+        atomicOr(&g_err_route, kErrBadIndex);
+      }
+      // every slot is written once: the row, or past the local experts' rows
+      // the sentinel n_token * topk the reference pre-fills permuted_idx with
+      a.pidx[dest] = dest < limit ? value : a.R;
+    }
+    __syncthreads();
+  }
+}
+
+// Single CTA of 1024 threads.  kOne: there is one chunk of keys, whose histogram
+// it makes itself (or finds, when the router left it) and which it scatters
+// too, in place of the two other kernels: three launches are what a few
+// tokens' routing takes its time for.  Dynamic smem then: wcnt[8][nb].
+template <bool kOne>
+__global__ void __launch_bounds__(1024) route_scan(RouteArgs a, int check_limit, int have_hist) {
   __shared__ int s_tot[kMaxBuckets];
   __shared__ int s_warp[32];
   const int tid = threadIdx.x;
   // 1) per-bucket exclusive scan across chunks (in place), bucket totals.
-  for (int b = tid; b < a.nb; b += 1024) {
+  if constexpr (kOne) {
+    extern __shared__ int s_wcnt[];
+    for (int b = tid; b < a.nb; b += 1024) s_tot[b] = have_hist ? a.hist[b] : 0;
+    for (int i = tid; i < 8 * a.nb; i += 1024) s_wcnt[i] = 0;
+    __syncthreads();
+    if (!have_hist)
+      for (int i = tid; i < a.R; i += 1024) atomicAdd(&s_tot[route_key(a, i)], 1);
+  }
+  for (int b = tid; !kOne && b < a.nb; b += 1024) {
     int run = 0;
     int c = 0;
     for (; c + 16 <= a.chunks; c += 16) {  // 16 loads in flight per thread
@@ -283,7 +339,7 @@ __global__ void __launch_bounds__(1024) route_scan(RouteArgs a) {
   __syncthreads();
   // 3) chunk bases become absolute destinations (8 loads in flight per
   // thread before the stores, not one round trip per entry).
-  {
+  if constexpr (!kOne) {
     const int total = a.chunks * a.nb;
     for (int i0 = tid; i0 < total; i0 += 8 * 1024) {
       int v[8];
@@ -350,6 +406,12 @@ __global__ void __launch_bounds__(1024) route_scan(RouteArgs a) {
     if (lo2 < E && lo2 + per2 >= E) a.so[E] = pre;
     if (E == 0 && tid == 0) a.so[0] = 0;
   }
+  if constexpr (kOne) {
+    extern __shared__ int s_wcnt[];
+    const int limit = check_limit ? s_tot[a.n_local] : a.R;
+    __syncthreads();  // s_tot counts up from here on
+    scatter_keys(a, 0, (a.R + kThreads - 1) / kThreads, s_tot, s_wcnt, limit);
+  }
 }
 
 // Stable scatter.  Dynamic smem: running[nb] + wcnt[8][nb].
@@ -357,47 +419,13 @@ __global__ void __launch_bounds__(kThreads) route_scatter(RouteArgs a, int check
   extern __shared__ int s_mem[];
   int* running = s_mem;
   int* wcnt = s_mem + a.nb;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x;
   const int* base = a.hist + static_cast<int64_t>(blockIdx.x) * a.nb;
   for (int b = tid; b < a.nb; b += kThreads) running[b] = base[b];
   for (int i = tid; i < 8 * a.nb; i += kThreads) wcnt[i] = 0;
   const int limit = check_limit ? static_cast<int>(a.eft[a.n_local]) : a.R;
   __syncthreads();
-  const unsigned lt_mask = (1u << lane) - 1u;
-  for (int j = 0; j < kKeysPerThread; ++j) {
-    const int i = blockIdx.x * kChunk + j * kThreads + tid;
-    const bool valid = i < a.R;
-    const int b = valid ? route_key(a, i) : a.nb;  // invalid lanes form their own group
-    const unsigned m = __match_any_sync(0xffffffffu, b);
-    const int rank = __popc(m & lt_mask);
-    const int cnt = __popc(m);
-    const bool leader = (m & lt_mask) == 0;
-    if (valid && leader) wcnt[warp * a.nb + b] = cnt;
-    __syncthreads();
-    int dest = 0;
-    if (valid) {
-      dest = running[b] + rank;
-      for (int w = 0; w < warp; ++w) dest += wcnt[w * a.nb + b];
-    }
-    __syncthreads();
-    if (valid && leader) {
-      atomicAdd(&running[b], cnt);
-      wcnt[warp * a.nb + b] = 0;
-    }
-    if (valid) {
-      // token_expert_indices is arange in the reference; null means exactly that
-      const int value = a.values != nullptr ? __ldg(a.values + i) : i;
-      if (value >= 0 && value < a.R) {
-        a.inv[value] = dest;
-      } else {
-        atomicOr(&g_err_route, kErrBadIndex);
-      }
-      // every slot is written once: the row, or past the local experts' rows
-      // the sentinel n_token * topk the reference pre-fills permuted_idx with
-      a.pidx[dest] = dest < limit ? value : a.R;
-    }
-    __syncthreads();
-  }
+  scatter_keys(a, blockIdx.x * kChunk, kKeysPerThread, running, wcnt, limit);
 }
 
 template <int VEC_BYTES>
@@ -553,6 +581,20 @@ int launch_route(const int32_t* topk_ids, const int32_t* tei, const int32_t* ema
     I8_CUDA(cudaFuncSetAttribute(route_scatter, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(smem_scatter)));
   }
+  if (chunks == 1) {
+    const size_t smem_one = 8 * nb * sizeof(int);
+    if (smem_one > 24 * 1024)  // with the static part, more than every kernel may have
+      I8_CUDA(cudaFuncSetAttribute(route_scan<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(smem_one)));
+    if (router != nullptr) {
+      const int vpl = router_vpl(router->E);
+      if (vpl == 8) router_kernel<8><<<1, kThreads, smem_hist, st>>>(*router, a);
+      else if (vpl == 16) router_kernel<16><<<1, kThreads, smem_hist, st>>>(*router, a);
+      else router_kernel<32><<<1, kThreads, smem_hist, st>>>(*router, a);
+    }
+    route_scan<true><<<1, 1024, smem_one, st>>>(a, emap != nullptr, router != nullptr);
+    return check_launch("route kernels");
+  }
   if (router != nullptr) {
     const int vpl = router_vpl(router->E);
     if (vpl == 8) router_kernel<8><<<chunks, kThreads, smem_hist, st>>>(*router, a);
@@ -561,7 +603,7 @@ int launch_route(const int32_t* topk_ids, const int32_t* tei, const int32_t* ema
   } else {
     route_hist<<<chunks, kThreads, smem_hist, st>>>(a);
   }
-  route_scan<<<1, 1024, 0, st>>>(a);
+  route_scan<false><<<1, 1024, 0, st>>>(a, 0, 1);
   route_scatter<<<chunks, kThreads, smem_scatter, st>>>(a, emap != nullptr ? 1 : 0);
   return check_launch("route kernels");
 }
