@@ -95,16 +95,31 @@ __device__ __forceinline__ int route_key(const RouteArgs& a, int i) {
   return route_key_of(a, __ldg(a.ids + i));
 }
 
+// The calling thread's keys of the chunk from key0 on, a.nb where there is none:
+// all loads are in flight together (one after the other, they were most of the
+// time of the histogram and of the scatter).
+__device__ __forceinline__ void load_keys(const RouteArgs& a, int key0, int (&key)[kKeysPerThread]) {
+  const int i0 = key0 + static_cast<int>(threadIdx.x);
+  const bool on = threadIdx.x < kThreads;
+#pragma unroll
+  for (int j = 0; j < kKeysPerThread; ++j) {
+    const int i = i0 + j * kThreads;
+    key[j] = on && i < a.R ? __ldg(a.ids + i) : 0;
+  }
+#pragma unroll
+  for (int j = 0; j < kKeysPerThread; ++j)
+    key[j] = on && i0 + j * kThreads < a.R ? route_key_of(a, key[j]) : a.nb;
+}
+
 __global__ void __launch_bounds__(kThreads) route_hist(RouteArgs a) {
   extern __shared__ int s_hist[];
   for (int b = threadIdx.x; b < a.nb; b += kThreads) s_hist[b] = 0;
   __syncthreads();
-  const int base = blockIdx.x * kChunk;
+  int key[kKeysPerThread];
+  load_keys(a, blockIdx.x * kChunk, key);
 #pragma unroll
-  for (int j = 0; j < kKeysPerThread; ++j) {
-    const int i = base + j * kThreads + threadIdx.x;
-    if (i < a.R) atomicAdd(&s_hist[route_key(a, i)], 1);
-  }
+  for (int j = 0; j < kKeysPerThread; ++j)
+    if (key[j] < a.nb) atomicAdd(&s_hist[key[j]], 1);
   __syncthreads();
   int* out = a.hist + static_cast<int64_t>(blockIdx.x) * a.nb;
   for (int b = threadIdx.x; b < a.nb; b += kThreads) out[b] = s_hist[b];
@@ -221,17 +236,21 @@ __global__ void __launch_bounds__(kThreads) router_kernel(RouterArgs r, RouteArg
   for (int b = threadIdx.x; b < a.nb; b += kThreads) out[b] = s_hist[b];
 }
 
-// Stable scatter of `rounds` x kThreads keys from key0 on, by the first kThreads
+// Stable scatter of the chunk of keys from key0 on, by the first kThreads
 // threads of a CTA (the others take part in the barriers): `running` holds each
 // bucket's next destination, wcnt [8][nb] zeros.
-__device__ __forceinline__ void scatter_keys(const RouteArgs& a, int key0, int rounds,
-                                             int* running, int* wcnt, int limit) {
+__device__ __forceinline__ void scatter_keys(const RouteArgs& a, int key0, int* running, int* wcnt,
+                                             int limit) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const unsigned lt_mask = (1u << lane) - 1u;
-  for (int j = 0; j < rounds; ++j) {
+  int key[kKeysPerThread];
+  load_keys(a, key0, key);
+#pragma unroll
+  for (int j = 0; j < kKeysPerThread; ++j) {
+    if (key0 + j * kThreads >= a.R) break;
     const int i = key0 + j * kThreads + tid;
-    const bool valid = tid < kThreads && i < a.R;
-    const int b = valid ? route_key(a, i) : a.nb;  // invalid lanes form their own group
+    const int b = key[j];  // invalid lanes form their own group
+    const bool valid = b < a.nb;
     const unsigned m = __match_any_sync(0xffffffffu, b);
     const int rank = __popc(m & lt_mask);
     const int cnt = __popc(m);
@@ -410,7 +429,7 @@ __global__ void __launch_bounds__(1024) route_scan(RouteArgs a, int check_limit,
     extern __shared__ int s_wcnt[];
     const int limit = check_limit ? s_tot[a.n_local] : a.R;
     __syncthreads();  // s_tot counts up from here on
-    scatter_keys(a, 0, (a.R + kThreads - 1) / kThreads, s_tot, s_wcnt, limit);
+    scatter_keys(a, 0, s_tot, s_wcnt, limit);
   }
 }
 
@@ -425,7 +444,7 @@ __global__ void __launch_bounds__(kThreads) route_scatter(RouteArgs a, int check
   for (int i = tid; i < 8 * a.nb; i += kThreads) wcnt[i] = 0;
   const int limit = check_limit ? static_cast<int>(a.eft[a.n_local]) : a.R;
   __syncthreads();
-  scatter_keys(a, blockIdx.x * kChunk, kKeysPerThread, running, wcnt, limit);
+  scatter_keys(a, blockIdx.x * kChunk, running, wcnt, limit);
 }
 
 template <int VEC_BYTES>
