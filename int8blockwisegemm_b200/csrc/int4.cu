@@ -682,6 +682,7 @@ int i8moe_quantize_weights_int4(const void* w, int dtype, int64_t n_expert, int6
   I8_REQUIRE(group_size == 32 || group_size == 64 || group_size == 128,
              "quantize_weights_int4: group_size must be 32, 64 or 128");
   if (n_expert == 0 || n == 0 || k == 0) return I8MOE_OK;
+  I8_REQUIRE(w && packed && scale, "quantize_weights_int4: every tensor must be given");
   const int groups = static_cast<int>((k + group_size - 1) / group_size);
   const int g = static_cast<int>(group_size);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -714,6 +715,8 @@ int i8moe_int4_grouped_mv(const void* x, int64_t x_stride, int64_t x_rows, int d
   I8_REQUIRE(permuted_idx != nullptr || x_rows >= n_rows,
              "int4_grouped_mv: x has fewer rows than the output");
   if (n_rows == 0 || n == 0 || n_expert == 0) return I8MOE_OK;
+  I8_REQUIRE(x && w_packed && w_scale && expert_offsets && out,
+             "int4_grouped_mv: every tensor must be given");
   I8_REQUIRE(x_stride >= k && x_stride % 8 == 0 && bits(x) % 16 == 0 && bits(w_packed) % 16 == 0 &&
                  bits(out) % 16 == 0,
              "int4_grouped_mv: x rows, w_packed and out must be 16-byte aligned");

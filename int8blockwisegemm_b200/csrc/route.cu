@@ -475,7 +475,8 @@ __global__ void __launch_bounds__(256, 6) unpermute_kernel(const T* __restrict__
   constexpr int EPV = 16 / sizeof(T);
   constexpr int G = 4;  // source rows in flight
   const int64_t t = blockIdx.x;
-  const int64_t valid = eft ? eft[n_local] : INT64_MAX;
+  const int64_t rows = static_cast<int64_t>(gridDim.x) * topk;
+  const int64_t valid = eft ? min(rows, static_cast<int64_t>(eft[n_local])) : rows;
   for (int v = threadIdx.x; v < vecs_per_row; v += blockDim.x) {
     float acc[EPV];
 #pragma unroll

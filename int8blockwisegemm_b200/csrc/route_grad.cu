@@ -11,6 +11,7 @@
 // inv is a permutation of the n_token * topk rows, so every row of P and dY
 // is written exactly once, and nothing is added in an order that varies.
 #include <algorithm>
+#include <initializer_list>
 
 #include "common.cuh"
 
@@ -129,9 +130,9 @@ __global__ void __launch_bounds__(256, 6) gather_sum_kernel(RowArgs a,
 
 // One token per CTA: its gradient is read once for all of its rows, four of
 // which are in flight, and their dot products are reduced together.  Bound by
-// memory: 8192 x 2048 bf16, top 8 (570 MB) takes about 92 us, 6.2 of the 6.6
-// TB/s of a copy; with eight rows in flight 120 us (registers for two CTAs an
-// SM only), with two 95.
+// memory: 8192 x 2048 bf16, top 8 (570 MB, half of it written) takes 100 us, 5.7
+// TB/s where a copy has 6.6; with eight rows in flight 125 us (registers for two
+// CTAs an SM only), with two 101.
 template <typename T>
 __global__ void __launch_bounds__(256, 4) return_grad_kernel(RowArgs a, const uint4* __restrict__ dout,
                                                           const uint4* __restrict__ rows,
@@ -197,7 +198,8 @@ __global__ void __launch_bounds__(256, 4) return_grad_kernel(RowArgs a, const ui
 
 // Checks shared by the entry points; fills `a`.
 int row_args(const char* what, int dtype, const int32_t* inv, const int64_t* eft, int64_t n_local,
-             int64_t n_token, int64_t topk, int64_t n_hidden, uintptr_t pointers, RowArgs* a) {
+             int64_t n_token, int64_t topk, int64_t n_hidden,
+             std::initializer_list<const void*> rows, RowArgs* a) {
   I8_REQUIRE(dtype == I8MOE_BF16 || dtype == I8MOE_FP16 || dtype == I8MOE_FP32,
              "%s: unsupported dtype", what);
   I8_REQUIRE(topk >= 1, "%s: topk must be positive", what);
@@ -206,14 +208,18 @@ int row_args(const char* what, int dtype, const int32_t* inv, const int64_t* eft
   I8_REQUIRE(n_hidden >= 0 && n_hidden < (int64_t(1) << 31), "%s: bad n_hidden", what);
   const int64_t row_bytes = n_hidden * (dtype == I8MOE_FP32 ? 4 : 2);
   I8_REQUIRE(row_bytes % 16 == 0, "%s: hidden row must be a multiple of 16 bytes", what);
-  I8_REQUIRE(pointers % 16 == 0, "%s: tensors must be 16-byte aligned", what);
+  if (n_token > 0 && n_hidden > 0)
+    for (const void* p : rows) {
+      I8_REQUIRE(p != nullptr, "%s: every tensor must be given", what);
+      I8_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0,
+                 "%s: tensors must be 16-byte aligned", what);
+    }
+  I8_REQUIRE(n_token == 0 || inv != nullptr, "%s: every tensor must be given", what);
   I8_REQUIRE(eft == nullptr || n_local >= 0, "%s: bad n_local_expert", what);
   *a = RowArgs{inv, eft, static_cast<int>(n_local), static_cast<int>(n_token),
                static_cast<int>(topk), static_cast<int>(row_bytes / 16)};
   return I8MOE_OK;
 }
-
-uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
 // Threads of a CTA for rows of that many vectors.
 int row_threads(int vpr) { return std::min(256, (vpr + 31) / 32 * 32); }
@@ -232,7 +238,7 @@ int i8moe_moe_scatter_rows(const void* input, int dtype, const int32_t* inv_perm
   RowArgs a;
   const int rc = row_args("moe_scatter_rows", dtype, inv_permuted_idx, expert_first_token_offset,
                           n_local_expert, n_token, topk, n_hidden,
-                          bits(input) | bits(permuted_input), &a);
+                          {input, permuted_input}, &a);
   if (rc != I8MOE_OK) return rc;
   if (n_token == 0 || n_hidden == 0) return I8MOE_OK;
   scatter_rows_kernel<<<static_cast<unsigned>(n_token), row_threads(a.vpr), 0,
@@ -249,7 +255,7 @@ int i8moe_moe_permute_backward(const void* permuted_grad, int dtype,
   RowArgs a;
   const int rc = row_args("moe_permute_backward", dtype, inv_permuted_idx,
                           expert_first_token_offset, n_local_expert, n_token, topk, n_hidden,
-                          bits(permuted_grad) | bits(input_grad), &a);
+                          {permuted_grad, input_grad}, &a);
   if (rc != I8MOE_OK) return rc;
   if (n_token == 0 || n_hidden == 0) return I8MOE_OK;
   const uint4* in = static_cast<const uint4*>(permuted_grad);
@@ -272,9 +278,10 @@ int i8moe_moe_unpermute_backward(const void* out_grad, const void* permuted_hidd
   const int rc =
       row_args("moe_unpermute_backward", dtype, inv_permuted_idx, expert_first_token_offset,
                n_local_expert, n_token, topk, n_hidden,
-               bits(out_grad) | bits(permuted_hidden) | bits(permuted_grad), &a);
+               {out_grad, permuted_hidden, permuted_grad}, &a);
   if (rc != I8MOE_OK) return rc;
   if (n_token == 0) return I8MOE_OK;
+  I8_REQUIRE(topk_weights && weights_grad, "moe_unpermute_backward: every tensor must be given");
   const uint4* g = static_cast<const uint4*>(out_grad);
   const uint4* y = static_cast<const uint4*>(permuted_hidden);
   uint4* dy = static_cast<uint4*>(permuted_grad);

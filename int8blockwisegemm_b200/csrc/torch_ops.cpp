@@ -6,6 +6,7 @@
 // address, so that INT8_HYBRID_MOE_LIB decides here too.
 #include <torch/extension.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -453,6 +454,7 @@ Tensor int4_grouped_mv(const Tensor& x_in, const Tensor& packed, const Tensor& s
                     out.size(1) == n_out && out.is_contiguous() && out.device() == device,
                 what,
                 ": out must be contiguous [rows, N (N/2 with silu)] of x's dtype on x's device");
+    at::assert_no_overlap(out, x_in);
   } else {
     out = empty({rows, n_out}, x_in, x_in.scalar_type());
   }

@@ -55,7 +55,7 @@ def int4_grouped_mv(x, w_packed, w_scale, expert_offsets, group_size: int = 128,
     gate rows and then N/2 up rows, and the result is silu(gate) * up.
     Returns ``out`` [rows, N] (N/2 with silu) in x's type, allocated when not
     given; rows outside every expert keep what it held.  Sums are fp32,
-    rounded once."""
+    rounded once.  No gradients."""
     return TORCH_OPS.int4_grouped_mv(x, w_packed, w_scale, expert_offsets, group_size, permuted_idx,
                                      topk, silu, out)
 
@@ -66,14 +66,19 @@ def run_int4_moe(output, hidden_states, w1_packed, w1_scale, w2_packed, w2_scale
     """MoE forward of a decoding step with 4-bit weights; writes ``output``
     [T, K].  w1 [E, 2N, K] (gate rows, then up rows) and w2 [E, K, N] as
     ``quantize_weights_int4`` packs them, E being the local experts;
-    ``expert_map`` as in the INT8 forward.  Six launches, no host
-    synchronisation; it can be captured into a CUDA graph."""
+    ``expert_map`` as in the INT8 forward.  Four launches for up to
+    2048 rows, six for more, no host synchronisation; it can be captured into
+    a CUDA graph."""
     _check(hidden_states.dim() == 2 and w1_packed.dim() == 3 and w2_packed.dim() == 3,
            "run_int4_moe: hidden_states must be [T, K], the weights [E, rows, columns / 2]")
     T, K = hidden_states.shape
     E, two_n, _ = w1_packed.shape
     _check(2 * w1_packed.size(2) == K and w2_packed.shape == (E, K, two_n // 4) and two_n % 4 == 0,
            "run_int4_moe: w1 must be [E, 2N, K] and w2 [E, K, N]")
+    _check(expert_map is None or (expert_map.dtype == torch.int32 and expert_map.is_contiguous()
+                                  and expert_map.shape == (global_num_experts,)
+                                  and expert_map.device == hidden_states.device),
+           "run_int4_moe: expert_map must be contiguous int32 [global_num_experts]")
     _check(topk_ids.dim() == 2 and topk_ids.size(0) == T and topk_weights.shape == topk_ids.shape,
            "run_int4_moe: topk_ids and topk_weights must have shape [T, topk]")
     _check(output.shape == hidden_states.shape and output.dtype == hidden_states.dtype

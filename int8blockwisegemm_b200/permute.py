@@ -157,7 +157,8 @@ def moe_permute_train(hidden_states, topk_ids, n_expert: int, n_local_expert: in
 
     Returns (permuted_hidden_states [T * topk, hidden],
     expert_first_token_offset, inv_permuted_idx (flat), permuted_idx); rows of
-    no local expert are zero and give no gradient."""
+    no local expert are zero and give no gradient.  topk_ids are in [0,
+    n_expert), or -1 for slots of no expert (without expert_map)."""
     return TORCH_OPS.moe_permute_train(hidden_states, topk_ids, n_expert, n_local_expert,
                                        expert_map)
 
@@ -165,8 +166,9 @@ def moe_permute_train(hidden_states, topk_ids, n_expert: int, n_local_expert: in
 def moe_unpermute_train(permuted_hidden_states, topk_weights, inv_permuted_idx,
                         expert_first_token_offset=None):
     """``moe_unpermute`` for training: returns [n_token, hidden],
-    differentiable in permuted_hidden_states and topk_weights (once).  Entries
-    of inv_permuted_idx must be rows."""
+    differentiable in permuted_hidden_states and topk_weights (once).
+    inv_permuted_idx is a permutation of the rows, as ``moe_permute_train`` and
+    the other routing calls give it."""
     return TORCH_OPS.moe_unpermute_train(permuted_hidden_states, topk_weights, inv_permuted_idx,
                                          expert_first_token_offset)
 
@@ -182,6 +184,7 @@ def moe_permute_backward(permuted_grad, inv_permuted_idx, expert_first_token_off
 def moe_unpermute_backward(out_grad, permuted_hidden_states, topk_weights, inv_permuted_idx,
                            expert_first_token_offset=None):
     """Gradients of ``moe_unpermute``: (of permuted_hidden_states, of
-    topk_weights in fp32); zero for rows of no local expert."""
+    topk_weights in fp32); zero for rows of no local expert.  inv_permuted_idx
+    is a permutation of the rows."""
     return TORCH_OPS.moe_unpermute_backward(out_grad, permuted_hidden_states, topk_weights,
                                             inv_permuted_idx, expert_first_token_offset)

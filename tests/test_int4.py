@@ -300,11 +300,22 @@ def test_refusals():
                           ((w[..., :40],), "divisible by 32"), ((w, 32, torch.int8), "dtype")]:
         with pytest.raises(RuntimeError, match=message):
             int4.quantize_weights_int4(*args)
+    square = weights(E, K, K, G, torch.bfloat16)
+    with pytest.raises(RuntimeError, match="single memory location"):
+        int4.int4_grouped_mv(x, *square, eo, G, out=x)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        int4.int4_grouped_mv(x.clone().requires_grad_(), packed, scale, eo, G)
+    odd = torch.empty(4 * N + 1, dtype=torch.bfloat16, device=DEV)[1:].view(4, N)
+    with pytest.raises(RuntimeError, match="16-byte aligned"):
+        int4.int4_grouped_mv(x, packed, scale, eo, G, out=odd)
     ids, wt = torch.zeros(4, 1, dtype=torch.int32, device=DEV), torch.ones(4, 1, device=DEV)
     w1, w2 = weights(E, 64, K, G, torch.bfloat16), weights(E, K, 32, G, torch.bfloat16)
     for out, a, message in [(x[:2], (*w1, *w2), "output"), (x, (*w2, *w2), "w1 must")]:
         with pytest.raises(RuntimeError, match=message):
             int4.run_int4_moe(out, x, *a, ids, wt, E, None, G)
+    with pytest.raises(RuntimeError, match="expert_map"):
+        int4.run_int4_moe(x.clone(), x, *w1, *w2, ids, wt, E, torch.zeros(E, device=DEV), G)
+    int4.run_int4_moe(x[:0].clone(), x[:0], *w1, *w2, ids[:0], wt[:0], E, None, G)  # no tokens: nothing to do
 
 
 def test_refuses_cpu_tensors():
@@ -328,7 +339,7 @@ def test_c_argument_errors_before_any_cuda_call():
                         (dict(n=15, silu=1), "bad N"), (dict(E=-1), "n_expert"), (dict(E=4096), "n_expert"),
                         (dict(rows=-1), "n_rows"), (dict(rows=5), "fewer rows"), (dict(topk=0, pidx=one), "topk"),
                         (dict(stride=32), "aligned"), (dict(stride=65), "aligned"),
-                        (dict(x=ctypes.c_void_p(8)), "aligned")]:
+                        (dict(x=ctypes.c_void_p(8)), "aligned"), (dict(x=None), "must be given")]:
         assert mv(**kw) == -1 and message in _lib.last_error(), kw
     assert mv(rows=0) == 0 and mv(n=0) == 0 and mv(E=0) == 0
 

@@ -211,6 +211,13 @@ def test_partial_gradients_and_unused_outputs():
     y = norm.rms_norm(x, w, 1e-6)
     y.sum().backward()  # an expanded gradient, weight alone
     assert x.grad is None and w.grad is not None
+    w.grad = None
+    one_row = torch.randn(64, device=DEV, requires_grad=True)  # no batch dimension
+    norm.rms_norm(one_row, w, 1e-6, one_row).__getitem__(0).sum().backward()  # its own residual
+    assert one_row.grad.shape == (64,) and w.grad.shape == (64,)
+    y = norm.rms_norm(r, w)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(y.sum(), r, create_graph=True)
     x = torch.zeros(0, 64, device=DEV, requires_grad=True)
     w.grad = None
     norm.rms_norm(x, w).sum().backward()

@@ -177,6 +177,8 @@ def test_layouts_and_partial_gradients():
     assert torch.equal(rows, want[0]) and dw.dtype == torch.bfloat16
     assert torch.equal(dw, want[7].to(torch.bfloat16))
     assert torch.equal(torch.autograd.grad(rows, x, c["drows"])[0], want[5])
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(permute.moe_permute_train(x, d["ids"], E)[0].sum(), x, create_graph=True)
     rows, *_ = permute.moe_permute_train(c["x"], c["ids"], E)
     assert not rows.requires_grad
     out = permute.moe_unpermute_train(c["y"], c["w"], inv)  # no offsets: every row counts
@@ -236,6 +238,10 @@ def test_bad_maps_are_reported():
     dx = permute.moe_permute_backward(c["drows"], inv, eft, 4, 2)
     assert torch.equal(dx[1], c["drows"][2]) and torch.equal(dx[2], c["drows"][4])
     assert _lib.device_error(0, clear=True) == 1 << 5
+    for offsets in (eft, None, eft * 100):  # rows past the tensor are not read
+        out = torch.empty(4, 64, device=DEV)
+        permute.moe_unpermute(out, c["y"], c["w"], inv, offsets)
+        assert torch.equal(out[1], c["w"][1, 0] * c["y"][2])
     _, dw = permute.moe_unpermute_backward(c["dout"], c["y"], c["w"], inv, eft)
     assert float(dw[1, 1]) == 0.0 and float(dw[2, 1]) == 0.0
     assert _lib.device_error(0, clear=True) == 1 << 5
@@ -286,6 +292,7 @@ def test_c_argument_errors_before_any_cuda_call():
                         (dict(n_token=1 << 40), "int32"), (dict(topk=0), "topk"), (dict(k=63), "16 bytes"),
                         (dict(k=-8), "n_hidden"), (dict(p=ctypes.c_void_p(8)), "aligned")]:
         assert calls(**kw) == [-1] * 3 and message in _lib.last_error(), kw
+    assert calls(p=None) == [-1] * 3 and "must be given" in _lib.last_error()
     assert calls(n_token=0) == [0] * 3
 
 
