@@ -8,8 +8,10 @@
 
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <initializer_list>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -80,6 +82,21 @@ Tensor empty(at::IntArrayRef size, const Tensor& like, at::ScalarType type) {
 // differentiable operators.
 void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once (no create_graph)");
+}
+
+// Inside a graph's capture: a leaf whose gradient node lives on in an eager
+// graph brings that graph's stream into the captured backward pass, which ends
+// the process there.  Refused here instead.
+void check_capture(const char* what, std::initializer_list<Tensor> inputs) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  for (const Tensor& t : inputs) {
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) continue;
+    const auto stream = node->stream();
+    TORCH_CHECK(!stream || *stream == at::cuda::getCurrentCUDAStream(t.get_device()).unwrap(), what,
+                ": an eager graph of the same leaves is alive; drop its outputs before capturing");
+  }
 }
 
 // ------------------------------------------------------------------- norm
@@ -202,6 +219,7 @@ py::object rms_norm(const Tensor& x, const Tensor& weight, double eps,
   check_norm("rms_norm", x, weight, eps, residual);
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || weight.requires_grad() || (residual && residual->requires_grad()))) {
+    check_capture("rms_norm", {x, weight, residual ? *residual : Tensor()});
     const variable_list out = RmsNorm::apply(x, weight, eps, residual);
     return residual ? py::cast(std::make_tuple(out[0], out[1])) : py::cast(out[0]);
   }
@@ -390,6 +408,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> moe_permute_train(const Tensor& x, co
                     emap->device() == x.device() && emap->dim() == 1 && emap->size(0) == n_expert,
                 what,
                 ": expert_map must be contiguous int32 [n_expert] on hidden_states' device");
+  if (at::GradMode::is_enabled()) check_capture(what, {x});
   const variable_list out =
       SortRows::apply(aligned(x), ids.to(at::kInt).contiguous(), emap, n_expert, n_local);
   return {out[0], out[1], out[2], out[3]};
@@ -405,6 +424,7 @@ Tensor moe_unpermute_train(const Tensor& rows, const Tensor& weights, const Tens
               ": permuted_hidden_states must have one row per element of topk_weights "
               "[n_token, topk]");
   check_maps(what, inv, eft, weights.numel(), rows);
+  if (at::GradMode::is_enabled()) check_capture(what, {rows, weights});
   return ReturnRows::apply(aligned(rows), weights.to(at::kFloat).contiguous(), inv, eft);
 }
 

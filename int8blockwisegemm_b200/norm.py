@@ -15,8 +15,9 @@ x is [..., K] in bf16, fp16 or fp32 on a CUDA device, of any K and alignment;
 rows may have any stride (a last dimension that is not contiguous is copied).
 ``weight`` is [K] in x's type or fp32; ``residual`` has x's shape and type.
 Outputs are new contiguous tensors; nothing synchronises with the host.  Both
-passes can be captured into a CUDA graph; as for every autograd graph, drop
-eager graphs that hold the same leaves before capturing a backward pass.
+passes can be captured into a CUDA graph; drop eager graphs that hold the same
+leaves before capturing a backward pass (a call on such a leaf is refused
+during capture).
 
 Arguments are checked in the compiled binding, which raises RuntimeError.
 """

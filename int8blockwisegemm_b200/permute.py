@@ -147,8 +147,8 @@ def moe_unpermute(out, permuted_hidden_states, topk_weights, inv_permuted_idx,
 
 # ---------------------------------------------------------------------------
 # Differentiable sort and return (extension).  Both passes can be captured into
-# a CUDA graph; as for every autograd graph, drop eager graphs that hold the
-# same leaves before capturing a backward pass.
+# a CUDA graph; drop eager graphs that hold the same leaves before capturing a
+# backward pass (a call on such a leaf is refused during capture).
 # ---------------------------------------------------------------------------
 
 def moe_permute_train(hidden_states, topk_ids, n_expert: int, n_local_expert: int = -1,

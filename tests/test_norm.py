@@ -273,6 +273,27 @@ def test_streams_and_graph_capture():
 
 
 @pytest.mark.gpu
+def test_capture_beside_an_eager_graph_is_refused():
+    """The captured backward pass would end the process; the call that would
+    lead to it raises, and the device goes on working."""
+    x = torch.randn(4, 64, device=DEV, requires_grad=True)
+    w = torch.ones(64, device=DEV)
+    eager = norm.rms_norm(x, w)
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            norm.rms_norm(x, w)
+    want = eager.detach().clone()
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = norm.rms_norm(x, w)
+        y.backward(torch.ones_like(y))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y.detach(), want) and x.grad.isfinite().all()
+
+
+@pytest.mark.gpu
 def test_refusals():
     x, w, r = make(4, 64, torch.bfloat16, torch.bfloat16, True)
     cases = [(dict(x=x.to(torch.float64)), "bfloat16, float16 or float32"),

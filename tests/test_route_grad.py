@@ -230,6 +230,20 @@ def test_streams_and_graph_capture():
 
 
 @pytest.mark.gpu
+def test_capture_beside_an_eager_graph_is_refused():
+    c = case(8, 64, 4, 4, 2, torch.float32)
+    x, y = c["x"].requires_grad_(), c["y"].requires_grad_()
+    rows, eft, inv, _ = permute.moe_permute_train(x, c["ids"], 4)
+    out = permute.moe_unpermute_train(y, c["w"], inv, eft)
+    for call in (lambda: permute.moe_permute_train(x, c["ids"], 4),
+                 lambda: permute.moe_unpermute_train(y, c["w"], inv, eft)):
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    assert rows.isfinite().all() and out.isfinite().all()
+
+
+@pytest.mark.gpu
 def test_bad_maps_are_reported():
     """Entries outside the rows are skipped and set the error bit."""
     c = case(4, 64, 4, 4, 2, torch.float32)
