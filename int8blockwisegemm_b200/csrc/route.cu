@@ -356,20 +356,10 @@ __global__ void __launch_bounds__(1024) route_scan(RouteArgs a, int check_limit,
     }
   }
   __syncthreads();
-  // 3) chunk bases become absolute destinations (8 loads in flight per
-  // thread before the stores, not one round trip per entry).
-  if constexpr (!kOne) {
-    const int total = a.chunks * a.nb;
-    for (int i0 = tid; i0 < total; i0 += 8 * 1024) {
-      int v[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (i0 + 1024 * u < total) v[u] = a.hist[i0 + 1024 * u];
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (i0 + 1024 * u < total) a.hist[i0 + 1024 * u] = v[u] + s_tot[(i0 + 1024 * u) % a.nb];
-    }
-  }
+  // 3) the buckets' first destinations, in the row of the first chunk, whose
+  // own counts before it are zero.
+  if constexpr (!kOne)
+    for (int b = tid; b < a.nb; b += 1024) a.hist[b] = s_tot[b];
   // 4) expert offsets (n_local < nb always).
   for (int e = tid; e <= a.n_local; e += 1024) {
     const int off = s_tot[e];
@@ -439,8 +429,9 @@ __global__ void __launch_bounds__(kThreads) route_scatter(RouteArgs a, int check
   int* running = s_mem;
   int* wcnt = s_mem + a.nb;
   const int tid = threadIdx.x;
-  const int* base = a.hist + static_cast<int64_t>(blockIdx.x) * a.nb;
-  for (int b = tid; b < a.nb; b += kThreads) running[b] = base[b];
+  const int* before = a.hist + static_cast<int64_t>(blockIdx.x) * a.nb;
+  for (int b = tid; b < a.nb; b += kThreads)
+    running[b] = a.hist[b] + (blockIdx.x > 0 ? before[b] : 0);
   for (int i = tid; i < 8 * a.nb; i += kThreads) wcnt[i] = 0;
   const int limit = check_limit ? static_cast<int>(a.eft[a.n_local]) : a.R;
   __syncthreads();
