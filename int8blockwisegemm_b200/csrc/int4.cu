@@ -42,6 +42,7 @@ struct MvArgs {
   const uint8_t* w;  // [E, N, K / 2]
   const void* scale;  // [E, N, groups], x's type
   int group, groups;
+  bool scale_packs;  // rows of scales hold whole steps, and start on 8 bytes
   const int32_t* eo;  // [E + 1]
   int n_expert;
   int64_t rows;
@@ -167,6 +168,11 @@ __device__ __forceinline__ void load_shared(uint32_t at, uint32_t* w) {
   else
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at));
 }
+
+template <typename T, int kCount>
+struct alignas(sizeof(T) * kCount) ScalePack {
+  T v[kCount];
+};
 
 // One CTA an SM: 12 warps of 158 registers take 62 us for the decode case's
 // first product, 16 of 128 (with spills) 70, 8 of 172 72.
@@ -337,6 +343,19 @@ __global__ void __launch_bounds__(kMvThreads, 1) mv_mma_kernel(MvArgs a) {
   };
   T s_next[2][kGroups];
   auto load_scales = [&](int step) {
+    // A step's scales of a row at once, where they are four: 83 instead of 124
+    // us for the decode case in groups of 32 (a load of every lane's own row is
+    // 32 lines to look up); two, in groups of 64, gain nothing (72 against 69).
+    if (kGroups == 4 && a.scale_packs) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const ScalePack<T, kGroups> p =
+            *reinterpret_cast<const ScalePack<T, kGroups>*>(s_set[h] + step * kGroups);
+#pragma unroll
+        for (int gi = 0; gi < kGroups; ++gi) s_next[h][gi] = p.v[gi];
+      }
+      return;
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -722,7 +741,8 @@ int i8moe_int4_grouped_mv(const void* x, int64_t x_stride, int64_t x_rows, int d
              "int4_grouped_mv: x rows, w_packed and out must be 16-byte aligned");
   MvArgs a{x, x_stride, x_rows, permuted_idx, static_cast<int>(topk), w_packed, w_scale,
            static_cast<int>(group_size),
-           static_cast<int>((k + group_size - 1) / group_size), expert_offsets,
+           static_cast<int>((k + group_size - 1) / group_size),
+           k % kMvStep == 0 && bits(w_scale) % 8 == 0, expert_offsets,
            static_cast<int>(n_expert), n_rows, static_cast<int>(n), static_cast<int>(k), out};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == I8MOE_BF16)
