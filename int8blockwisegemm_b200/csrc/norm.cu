@@ -78,6 +78,56 @@ __device__ __forceinline__ void load_weight(const void* w, int dtype, int i, flo
   }
 }
 
+// The same one by one, 0 outside of the row.
+template <int kVec, typename W>
+__device__ __forceinline__ void load_elements(const W* w, int i, int k, float* out) {
+  if (i >= 0 && i + kVec <= k) {
+    w += i;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) out[e] = Num<W>::to_f(w[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      out[e] = Num<W>::to_f(w[min(max(i + e, 0), k - 1)]);
+      if (i + e < 0 || i + e >= k) out[e] = 0.f;
+    }
+  }
+}
+// The elements from i on, shift elements before a 16-byte boundary: cut out of
+// the two packs that hold them (8192 x 1001: 21 instead of 25 us one by one).
+template <typename T, int kVec>
+__device__ __forceinline__ void load_weight_at(const void* w, int dtype, int i, int shift, int k,
+                                               float* out) {
+  if constexpr (sizeof(T) < 4) {
+    if (dtype != I8MOE_FP32) {
+      const T* p = static_cast<const T*>(w);
+      const int up = i + shift;  // of the two packs that hold the elements, the second
+      if (up + kVec > k || reinterpret_cast<uintptr_t>(w) % 16 != 0) {
+        load_elements<kVec>(p, i, k, out);
+        return;
+      }
+      const uint4 hi = *reinterpret_cast<const uint4*>(p + up);
+      uint4 lo = make_uint4(0, 0, 0, 0);
+      if (up > 0) lo = *reinterpret_cast<const uint4*>(p + up - kVec);
+      uint32_t d[9] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w, 0};
+      const int at = kVec - shift;  // the first element's place in both
+#pragma unroll
+      for (int step = 8; step >= 2; step /= 2)
+#pragma unroll
+        for (int j = 0; j < 9; ++j)
+          if (at & step) d[j] = j + step / 2 < 9 ? d[j + step / 2] : 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t v = __funnelshift_r(d[j], d[j + 1], at & 1 ? 16 : 0);
+        out[2 * j] = Num<T>::to_f(reinterpret_cast<const T*>(&v)[0]);
+        out[2 * j + 1] = Num<T>::to_f(reinterpret_cast<const T*>(&v)[1]);
+      }
+      return;
+    }
+  }
+  load_elements<kVec>(static_cast<const float*>(w), i, k, out);
+}
+
 // max that keeps NaN, so that a row without a finite norm gets a NaN scale
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -122,7 +172,8 @@ struct Int8Row {
 };
 __device__ __forceinline__ Int8Row int8_row(float largest) {
   const bool finite = largest < __int_as_float(0x7f800000);
-  return {finite ? __fdividef(127.f, largest) : 0.f, static_cast<uint8_t>(finite ? 0xff : 0)};
+  // scaled, because the fast division gives 0 for a divisor above 2^126
+  return {finite ? __fdividef(127.f / 256, largest * (1.f / 256)) : 0.f, static_cast<uint8_t>(finite ? 0xff : 0)};
 }
 
 // kVec elements that one thread reads or writes at once.
@@ -131,75 +182,128 @@ struct alignas(sizeof(T) * kVec) Pack {
   T v[kVec];
 };
 
+// Rows whose width no pack divides (kShift in the kernels): where every tensor
+// starts on 16 bytes and its stride leaves the same remainder as the width, row
+// r begins shift_of(r, k) elements behind a 16-byte boundary in all of them, so
+// that packs counted from that boundary are aligned everywhere; the first and
+// the last one reach over the row's ends.  Only the weight is off by the shift.
+// 4096 x 2047 bf16 with a residual: 23 us instead of 31 element by element,
+// with its gradients 55 instead of 74.
+template <int kVec>
+__device__ __forceinline__ int shift_of(int64_t r, int k) {
+  return static_cast<int>((static_cast<uint32_t>(r) * static_cast<uint32_t>(k)) % kVec);
+}
+
+// Zeros the elements outside of the row.
+template <typename T, int kVec>
+__device__ __forceinline__ void trim(Pack<T, kVec>& v, int i, int k) {
+#pragma unroll
+  for (int e = 0; e < kVec; ++e)
+    if (i + e < 0 || i + e >= k) v.v[e] = Num<T>::from_f(0.f);
+}
+
+// row[i, i + kVec), of which only what lies in [0, k)
+template <bool kShift, typename T, int kVec>
+__device__ __forceinline__ void store_pack(T* row, int i, int k, const Pack<T, kVec>& v) {
+  if (!kShift || (i >= 0 && i + kVec <= k)) {
+    *reinterpret_cast<Pack<T, kVec>*>(row + i) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e)
+      if (i + e >= 0 && i + e < k) row[i + e] = v.v[e];
+  }
+}
+
 // Rows in registers: blockDim.x threads hold a row, kPer packs each (a CTA has
 // several rows where a row takes less than a warp), so that it is read once,
 // and the sum of squares and the largest |h * weight| (from which the int8
 // scale follows, rstd being one factor of the row) are reduced together.  kVec
-// is 16 bytes' worth when width, strides and pointers allow it, else 1.
+// is 16 bytes' worth when width, strides and pointers allow it, with kShift or
+// without, else 1.
 // Bound by memory: 8192 x 2048 bf16 with a residual takes 26 us, 5.2 TB/s of
-// the 6.6 that a copy has; with two packs a thread 27, with four 30.
-template <typename T, int kVec, int kPer>
+// the 6.6 that a copy has; with two packs a thread 27, with four 30, with CTAs
+// that stay and load the next row ahead 31.
+template <typename T, int kVec, int kPer, bool kShift, bool kQuant>
 __global__ void __launch_bounds__(1024) norm_row_kernel(NormArgs a) {
   using P = Pack<T, kVec>;
   __shared__ float s_sum[32], s_max[32];
   const int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const int k = r < a.rows ? a.k : 0;
   const int tid = threadIdx.x, stride = blockDim.x * kVec;
+  const int shift = kShift ? shift_of<kVec>(r, a.k) : 0, first = tid * kVec - shift;
   const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
   const T* res = static_cast<const T*>(a.residual) + r * a.residual_stride;
   P xv[kPer], rv[kPer];
+#pragma unroll
+  for (int p = 0; p < kPer; ++p) {
+    const int i = p * stride + first;
+    if (i < k) {
+      // what lies before a row, or behind one that is not the last, belongs to the tensor too
+      if (!kShift || i + kVec <= k || r + 1 < a.rows) {
+        xv[p] = *reinterpret_cast<const P*>(x + i);
+        if (a.residual) rv[p] = *reinterpret_cast<const P*>(res + i);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          if (i + e >= 0 && i + e < k) {
+            xv[p].v[e] = x[i + e];
+            if (a.residual) rv[p].v[e] = res[i + e];
+          }
+        }
+      }
+    }
+  }
   float w[kPer][kVec];
 #pragma unroll
   for (int p = 0; p < kPer; ++p) {
-    const int i = p * stride + tid * kVec;
+    const int i = p * stride + first;
     if (i < k) {
-      xv[p] = *reinterpret_cast<const P*>(x + i);
-      if (a.residual) rv[p] = *reinterpret_cast<const P*>(res + i);
+      if constexpr (kShift) load_weight_at<T, kVec>(a.weight, a.weight_dtype, i, shift, k, w[p]);
+      else load_weight<T, kVec>(a.weight, a.weight_dtype, i, w[p]);
     }
-  }
-#pragma unroll
-  for (int p = 0; p < kPer; ++p) {
-    const int i = p * stride + tid * kVec;
-    if (i < k) load_weight<T, kVec>(a.weight, a.weight_dtype, i, w[p]);
   }
   float h[kPer][kVec];
   float ss = 0.f, m = 0.f;
 #pragma unroll
   for (int p = 0; p < kPer; ++p) {
-    const int i = p * stride + tid * kVec;
+    const int i = p * stride + first;
     if (i < k) {
+      if (kShift && (i < 0 || i + kVec > k)) {
+        trim(xv[p], i, k);
+        if (a.residual) trim(rv[p], i, k);
+      }
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
         h[p][e] = Num<T>::to_f(xv[p].v[e]);
         if (a.residual) h[p][e] += Num<T>::to_f(rv[p].v[e]);
         ss = fmaf(h[p][e], h[p][e], ss);
-        m = max_nan(m, fabsf(h[p][e] * w[p][e]));
+        if constexpr (kQuant) m = max_nan(m, fabsf(h[p][e] * w[p][e]));
       }
       if (a.h) {
         P o;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) o.v[e] = Num<T>::from_f(h[p][e]);
-        *reinterpret_cast<P*>(static_cast<T*>(a.h) + r * a.k + i) = o;
+        store_pack<kShift>(static_cast<T*>(a.h) + r * a.k, i, k, o);
       }
     }
   }
   for (int o = min(32, static_cast<int>(blockDim.x)) >> 1; o > 0; o >>= 1) {
     ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if constexpr (kQuant) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   }
   if (blockDim.x > 32) {  // one row
     if ((tid & 31) == 0) {
       s_sum[tid >> 5] = ss;
-      s_max[tid >> 5] = m;
+      if constexpr (kQuant) s_max[tid >> 5] = m;
     }
     __syncthreads();
     const bool on = (tid & 31) < (blockDim.x >> 5);
     ss = on ? s_sum[tid & 31] : 0.f;
-    m = on ? s_max[tid & 31] : 0.f;
+    if constexpr (kQuant) m = on ? s_max[tid & 31] : 0.f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if constexpr (kQuant) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     }
   }
   const float rstd = rsqrtf(fmaf(ss, a.inv_k, a.eps));
@@ -207,26 +311,25 @@ __global__ void __launch_bounds__(1024) norm_row_kernel(NormArgs a) {
   const Int8Row row = int8_row(largest);
   if (tid == 0 && k > 0) {
     if (a.rstd) a.rstd[r] = rstd;
-    if (a.q) a.scale[r] = largest / 127.f;
+    if constexpr (kQuant) a.scale[r] = largest / 127.f;
   }
 #pragma unroll
   for (int p = 0; p < kPer; ++p) {
-    const int i = p * stride + tid * kVec;
+    const int i = p * stride + first;
     if (i < k) {
-      float y[kVec];
+      P o;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) y[e] = h[p][e] * rstd * w[p][e];
-      if (a.y) {
-        P o;
+      for (int e = 0; e < kVec; ++e) h[p][e] = h[p][e] * rstd * w[p][e];
+      if (!kQuant || a.y) {
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) o.v[e] = Num<T>::from_f(y[e]);
-        *reinterpret_cast<P*>(static_cast<T*>(a.y) + r * a.k + i) = o;
+        for (int e = 0; e < kVec; ++e) o.v[e] = Num<T>::from_f(h[p][e]);
+        store_pack<kShift>(static_cast<T*>(a.y) + r * a.k, i, k, o);
       }
-      if (a.q) {
-        Pack<int8_t, kVec> o;
+      if constexpr (kQuant) {
+        Pack<int8_t, kVec> q;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) o.v[e] = to_int8(y[e], row.inv) & row.mask;
-        *reinterpret_cast<Pack<int8_t, kVec>*>(a.q + r * a.k + i) = o;
+        for (int e = 0; e < kVec; ++e) q.v[e] = to_int8(h[p][e], row.inv) & row.mask;
+        store_pack<kShift>(a.q + r * a.k, i, k, q);
       }
     }
   }
@@ -290,14 +393,15 @@ struct NormGradArgs {
 };
 
 template <int kPer>
-constexpr int kGradStages = kPer > 2 ? 1 : 3;  // rows of a group in shared memory
+constexpr int kGradStages = kPer > 2 ? 1 : 2;  // rows of a group in shared memory
 // Threads of a CTA whose groups have that many, and CTAs resident on an SM:
 // 768 threads of 80 registers (1024 of 64 spilled: 52 instead of 36 us), for
-// one group of 512 threads 1024, for more packs a thread 512.
+// one group of 512 threads 1024, for more packs a thread 512, and for shifted
+// rows, which take more registers, 512 (8192 x 1001: 28 instead of 38 us).
 template <int kThreads>
 constexpr int kGradThreads = kThreads > 256 ? kThreads : 256;
-template <int kVec, int kPer, int kThreads>
-constexpr int kGradCtas = kThreads <= 256 ? 3 : kPer <= (kVec == 1 ? 4 : 1) ? 2 : 1;
+template <int kVec, int kPer, int kThreads, bool kShift>
+constexpr int kGradCtas = kThreads <= 256 ? (kShift ? 2 : 3) : kPer <= (kVec == 1 ? 4 : 1) ? 2 : 1;
 // The most CTAs of a backward pass, and partial sums of the weight's gradient
 // that it writes (one row of k each) before they are added up.
 constexpr int kNormParts = 444;
@@ -308,11 +412,13 @@ constexpr int kNormParts = 444;
 // memory, of which every thread reads what it copied itself, so that the next
 // rows are on their way during a row's one reduction (one barrier of the
 // group; the halves of s_part take turns) without holding registers: with the
-// next row in registers instead, the default size took 48 us, spills and all.
+// next row in registers instead, the default size took 48 us, spills and all;
+// a third row in the ring costs 1 us.
 // Single elements (kVec 1) do wait in registers, of which they take few.  A
-// CTA's groups meet at its end.  The grid is what is resident at once.
-template <typename T, int kVec, int kPer, int kThreads, bool kWeight>
-__global__ void __launch_bounds__(kGradThreads<kThreads>, kGradCtas<kVec, kPer, kThreads>)
+// CTA's groups meet at its end.  The grid is what is resident at once; with
+// kShift a multiple of 8, so that all rows of a CTA have the same shift.
+template <typename T, int kVec, int kPer, int kThreads, bool kWeight, bool kShift>
+__global__ void __launch_bounds__(kGradThreads<kThreads>, kGradCtas<kVec, kPer, kThreads, kShift>)
     norm_grad_row_kernel(NormGradArgs a) {
   using P = Pack<T, kVec>;
   constexpr int kCta = kGradThreads<kThreads>;
@@ -325,6 +431,7 @@ __global__ void __launch_bounds__(kGradThreads<kThreads>, kGradCtas<kVec, kPer, 
   const int lane = tid & 31;
   const int64_t rows_at_once = static_cast<int64_t>(gridDim.x) * kGroups;
   int64_t r = static_cast<int64_t>(group) * gridDim.x + blockIdx.x;
+  const int shift = kShift ? shift_of<kVec>(r, a.k) : 0, first = tid * kVec - shift;
   auto row_of = [&](int which, int64_t row) {
     return which == 0   ? static_cast<const T*>(a.x) + row * a.x_stride
            : which == 1 ? static_cast<const T*>(a.dy) + row * a.dy_stride
@@ -344,22 +451,23 @@ __global__ void __launch_bounds__(kGradThreads<kThreads>, kGradCtas<kVec, kPer, 
         if (there(which))
 #pragma unroll
           for (int p = 0; p < kPer; ++p) {
-            const int i = (p * kThreads + tid) * kVec;
-            if (i < a.k)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+            const int i = p * (kThreads * kVec) + first;
+            if (i < a.k)  // zeros behind the row; what lies before it belongs to the tensor too
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                                smem_u32(ring(stage, which, p))),
-                           "l"(row_of(which, row) + i)
+                           "l"(row_of(which, row) + i),
+                           "r"(kShift ? min(kVec, a.k - i) * static_cast<int>(sizeof(T)) : 16)
                            : "memory");
           }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  P now[kRing ? 1 : 4][kPer], next[kRing ? 1 : 4][kPer];
+  P now[kRing ? 1 : 4][kPer] = {}, next[kRing ? 1 : 4][kPer] = {};
   auto load = [&](int64_t row) {
 #pragma unroll
     for (int which = 0; which < 4; ++which)
 #pragma unroll
       for (int p = 0; p < kPer; ++p) {
-        const int i = (p * kThreads + tid) * kVec;
+        const int i = p * (kThreads * kVec) + first;
         if (i < a.k && there(which))
           next[kRing ? 0 : which][p] = *reinterpret_cast<const P*>(row_of(which, row) + i);
       }
@@ -378,8 +486,11 @@ __global__ void __launch_bounds__(kGradThreads<kThreads>, kGradCtas<kVec, kPer, 
   float w[kPer][kVec], dw[kPer][kVec];
 #pragma unroll
   for (int p = 0; p < kPer; ++p) {
-    const int i = (p * kThreads + tid) * kVec;
-    if (i < a.k) load_weight<T, kVec>(a.weight, a.weight_dtype, i, w[p]);
+    const int i = p * (kThreads * kVec) + first;
+    if (i < a.k) {
+      if constexpr (kShift) load_weight_at<T, kVec>(a.weight, a.weight_dtype, i, shift, a.k, w[p]);
+      else load_weight<T, kVec>(a.weight, a.weight_dtype, i, w[p]);
+    }
 #pragma unroll
     for (int e = 0; e < kVec; ++e) dw[p][e] = 0.f;
   }
@@ -389,6 +500,11 @@ __global__ void __launch_bounds__(kGradThreads<kThreads>, kGradCtas<kVec, kPer, 
     if (r + rows_at_once < a.rows) rstd_next = a.rstd[r + rows_at_once];
     if constexpr (kRing) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      if (kShift && first < 0) {
+#pragma unroll
+        for (int which = 0; which < 3; ++which)
+          if (there(which)) trim(*reinterpret_cast<P*>(ring(stage, which, 0)), first, a.k);
+      }
     } else {
 #pragma unroll
       for (int which = 0; which < 4; ++which)
@@ -399,7 +515,7 @@ __global__ void __launch_bounds__(kGradThreads<kThreads>, kGradCtas<kVec, kPer, 
     float dot = 0.f;  // of dy * weight and h
 #pragma unroll
     for (int p = 0; p < kPer; ++p) {
-      const int i = (p * kThreads + tid) * kVec;
+      const int i = p * (kThreads * kVec) + first;
       if (i < a.k) {
         const P x = get(stage, 0, p), g = get(stage, 1, p);
         P res;
@@ -428,7 +544,7 @@ __global__ void __launch_bounds__(kGradThreads<kThreads>, kGradCtas<kVec, kPer, 
     const float back = -(rstd * rstd) * (rstd * (dot * a.inv_k));
 #pragma unroll
     for (int p = 0; p < kPer; ++p) {
-      const int i = (p * kThreads + tid) * kVec;
+      const int i = p * (kThreads * kVec) + first;
       if (i < a.k) {
         const P x = get(stage, 0, p), g = get(stage, 1, p);
         P o, res, add;
@@ -443,7 +559,7 @@ __global__ void __launch_bounds__(kGradThreads<kThreads>, kGradCtas<kVec, kPer, 
           if (a.dh) d += Num<T>::to_f(add.v[e]);
           o.v[e] = Num<T>::from_f(d);
         }
-        *reinterpret_cast<P*>(static_cast<T*>(a.dx) + r * a.k + i) = o;
+        store_pack<kShift>(static_cast<T*>(a.dx) + r * a.k, i, a.k, o);
       }
     }
     if constexpr (kRing) {
@@ -468,14 +584,15 @@ __global__ void __launch_bounds__(kGradThreads<kThreads>, kGradCtas<kVec, kPer, 
     }
 #pragma unroll
     for (int p = 0; p < kPer; ++p) {
-      const int i = (p * kThreads + tid) * kVec;
+      const int i = p * (kThreads * kVec) + first;
       if (i < a.k)
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
           float v = dw[p][e];
           for (int o = 0; o < kGroups - 1; ++o)
             v += s_dw[(o * kPer * kVec + p * kVec + e) * kThreads + tid];
-          a.part[static_cast<int64_t>(blockIdx.x) * a.k + i + e] = v;
+          if (!kShift || (i + e >= 0 && i + e < a.k))
+            a.part[static_cast<int64_t>(blockIdx.x) * a.k + i + e] = v;
         }
     }
   }
@@ -553,37 +670,57 @@ bool float_dtype(int d) { return d == I8MOE_BF16 || d == I8MOE_FP16 || d == I8MO
 
 uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
-template <typename T, int kVec, int kPer>
+// Whether rows can be read by shifted packs: k and the strides leave the same
+// remainder, and a row's ends lie inside the rows beside it.
+template <int kVec>
+bool same_shift(int k, int64_t stride) { return stride >= k && stride % kVec == k % kVec; }
+
+// Columns that the threads of a row have to cover.
+template <int kVec, bool kShift>
+constexpr int covered(int k) { return k + (kShift ? kVec - 1 : 0); }
+
+template <typename T, int kVec, int kPer, bool kShift>
 void launch_norm_row(const NormArgs& a, cudaStream_t st) {
-  const int need = (a.k + kVec * kPer - 1) / (kVec * kPer);
+  const int need = (covered<kVec, kShift>(a.k) + kVec * kPer - 1) / (kVec * kPer);
   int x = 1;
   while (x < 32 && x < need) x *= 2;
   if (need > 32) x = (need + 31) / 32 * 32;
   const int y = x <= 32 ? 128 / x : 1;
-  norm_row_kernel<T, kVec, kPer>
-      <<<static_cast<unsigned>((a.rows + y - 1) / y), dim3(x, y), 0, st>>>(a);
+  auto kernel = a.q ? norm_row_kernel<T, kVec, kPer, kShift, true>
+                    : norm_row_kernel<T, kVec, kPer, kShift, false>;
+  kernel<<<static_cast<unsigned>((a.rows + y - 1) / y), dim3(x, y), 0, st>>>(a);
 }
 
 // One pack a thread while that makes no CTA of more than 512 threads; elements
 // one by one come eight to a thread (4096 x 2047 bf16: 33 us with four, 41
 // with two).
-template <typename T, int kVec>
+template <typename T, int kVec, bool kShift>
 bool launch_norm_rows(const NormArgs& a, cudaStream_t st) {
-  if (kVec == 1 && a.k <= 8 * 1024) launch_norm_row<T, 1, 8>(a, st);
-  else if (kVec > 1 && a.k <= kVec * 512) launch_norm_row<T, kVec, 1>(a, st);
-  else if (kVec > 1 && a.k <= kVec * 2 * 1024) launch_norm_row<T, kVec, 2>(a, st);
-  else return false;
+  const int k = covered<kVec, kShift>(a.k);
+  if constexpr (kVec == 1) {
+    if (k > 8 * 1024) return false;
+    launch_norm_row<T, 1, 8, false>(a, st);
+  } else if (k <= kVec * 512) {
+    launch_norm_row<T, kVec, 1, kShift>(a, st);
+  } else if (k <= kVec * 2 * 1024) {
+    launch_norm_row<T, kVec, 2, kShift>(a, st);
+  } else {
+    return false;
+  }
   return true;
 }
 
 template <typename T>
 int launch_norm(const NormArgs& a, cudaStream_t st) {
   constexpr int kVec = 16 / sizeof(T);
-  const bool packs =
-      a.k % kVec == 0 && a.x_stride % kVec == 0 && (!a.residual || a.residual_stride % kVec == 0) &&
-      (bits(a.x) | bits(a.residual) | bits(a.weight) | bits(a.h) | bits(a.y)) % 16 == 0 &&
-      bits(a.q) % 8 == 0;
-  if (!(packs ? launch_norm_rows<T, kVec>(a, st) : launch_norm_rows<T, 1>(a, st))) {
+  const bool aligned = (bits(a.x) | bits(a.residual) | bits(a.h) | bits(a.y)) % 16 == 0 && bits(a.q) % 8 == 0;
+  const bool packs = aligned && bits(a.weight) % 16 == 0 && a.k % kVec == 0 && a.x_stride % kVec == 0 &&
+                     (!a.residual || a.residual_stride % kVec == 0);
+  const bool shift = aligned && a.k >= kVec && same_shift<kVec>(a.k, a.x_stride) &&
+                     (!a.residual || same_shift<kVec>(a.k, a.residual_stride));
+  if (!(packs   ? launch_norm_rows<T, kVec, false>(a, st)
+        : shift ? launch_norm_rows<T, kVec, true>(a, st)
+                : launch_norm_rows<T, 1, false>(a, st))) {
     const int sms = num_sms(current_device());
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, sms * 8));
     norm_wide_kernel<T><<<grid, 256, 0, st>>>(a);
@@ -591,17 +728,18 @@ int launch_norm(const NormArgs& a, cudaStream_t st) {
   return check_launch("rms_norm");
 }
 
-template <typename T, int kVec, int kPer, int kThreads>
+template <typename T, int kVec, bool kShift, int kPer, int kThreads>
 int launch_norm_grad_kernel(NormGradArgs& a, cudaStream_t st) {
   constexpr int kCta = kGradThreads<kThreads>, kGroups = kCta / kThreads;
-  const int64_t most = int64_t(num_sms(current_device())) * kGradCtas<kVec, kPer, kThreads>;
+  const int64_t most = int64_t(num_sms(current_device())) * kGradCtas<kVec, kPer, kThreads, kShift>;
   a.n_part = static_cast<int>(
       std::min({(a.rows + kGroups - 1) / kGroups, most, int64_t(kNormParts)}));
+  if (kShift) a.n_part -= a.n_part % 8;
   constexpr int kRing = kVec > 1 ? kGradStages<kPer> * 4 * kPer * kCta * 16 : 0;
   constexpr int kMeet = (kGroups - 1) * kPer * kVec * kThreads * 4;
   constexpr int kSmem = kRing > kMeet ? kRing : kMeet;
-  auto kernel = a.part ? norm_grad_row_kernel<T, kVec, kPer, kThreads, true>
-                       : norm_grad_row_kernel<T, kVec, kPer, kThreads, false>;
+  auto kernel = a.part ? norm_grad_row_kernel<T, kVec, kPer, kThreads, true, kShift>
+                       : norm_grad_row_kernel<T, kVec, kPer, kThreads, false, kShift>;
   if (kSmem > 40 * 1024)  // with the static part, more than every kernel may have
     I8_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   kernel<<<a.n_part, kCta, kSmem, st>>>(a);
@@ -609,17 +747,17 @@ int launch_norm_grad_kernel(NormGradArgs& a, cudaStream_t st) {
 }
 
 // Widths that fit a CTA's registers; `*wide` says that this one does not.
-template <typename T, int kVec>
+template <typename T, int kVec, bool kShift>
 int launch_norm_grad_rows(NormGradArgs& a, cudaStream_t st, bool* wide) {
   constexpr int kMost = kVec == 1 ? 8 : kVec == 4 ? 4 : 2;  // what the registers hold
-  const int packs = (a.k + kVec - 1) / kVec;
-  if (packs <= 32) return launch_norm_grad_kernel<T, kVec, 1, 32>(a, st);
-  if (packs <= 64) return launch_norm_grad_kernel<T, kVec, 1, 64>(a, st);
-  if (packs <= 128) return launch_norm_grad_kernel<T, kVec, 1, 128>(a, st);
-  if (packs <= 256) return launch_norm_grad_kernel<T, kVec, 1, 256>(a, st);
-  if (packs <= 512) return launch_norm_grad_kernel<T, kVec, 1, 512>(a, st);
-  if (packs <= 1024) return launch_norm_grad_kernel<T, kVec, 2, 512>(a, st);
-  if (packs <= 512 * kMost) return launch_norm_grad_kernel<T, kVec, kMost, 512>(a, st);
+  const int packs = (covered<kVec, kShift>(a.k) + kVec - 1) / kVec;
+  if (packs <= 32) return launch_norm_grad_kernel<T, kVec, kShift, 1, 32>(a, st);
+  if (packs <= 64) return launch_norm_grad_kernel<T, kVec, kShift, 1, 64>(a, st);
+  if (packs <= 128) return launch_norm_grad_kernel<T, kVec, kShift, 1, 128>(a, st);
+  if (packs <= 256) return launch_norm_grad_kernel<T, kVec, kShift, 1, 256>(a, st);
+  if (packs <= 512) return launch_norm_grad_kernel<T, kVec, kShift, 1, 512>(a, st);
+  if (packs <= 1024) return launch_norm_grad_kernel<T, kVec, kShift, 2, 512>(a, st);
+  if (packs <= 512 * kMost) return launch_norm_grad_kernel<T, kVec, kShift, kMost, 512>(a, st);
   *wide = true;
   return I8MOE_OK;
 }
@@ -627,14 +765,21 @@ int launch_norm_grad_rows(NormGradArgs& a, cudaStream_t st, bool* wide) {
 template <typename T>
 int launch_norm_grad(NormGradArgs& a, cudaStream_t st) {
   constexpr int kVec = 16 / sizeof(T);
-  const bool packs = a.k % kVec == 0 && a.x_stride % kVec == 0 && a.dy_stride % kVec == 0 &&
+  const bool aligned =
+      (bits(a.x) | bits(a.residual) | bits(a.dy) | bits(a.dh) | bits(a.dx)) % 16 == 0;
+  const bool packs = aligned && bits(a.weight) % 16 == 0 && a.k % kVec == 0 &&
+                     a.x_stride % kVec == 0 && a.dy_stride % kVec == 0 &&
                      (!a.residual || a.residual_stride % kVec == 0) &&
-                     (!a.dh || a.dh_stride % kVec == 0) &&
-                     (bits(a.x) | bits(a.residual) | bits(a.dy) | bits(a.dh) | bits(a.weight) |
-                      bits(a.dx)) % 16 == 0;
+                     (!a.dh || a.dh_stride % kVec == 0);
+  // 64 rows: eight CTAs, each with a row for the most groups that it may have
+  const bool shift = aligned && a.rows >= 64 && a.k >= kVec && same_shift<kVec>(a.k, a.x_stride) &&
+                     same_shift<kVec>(a.k, a.dy_stride) &&
+                     (!a.residual || same_shift<kVec>(a.k, a.residual_stride)) &&
+                     (!a.dh || same_shift<kVec>(a.k, a.dh_stride));
   bool wide = false;
-  const int rc = packs ? launch_norm_grad_rows<T, kVec>(a, st, &wide)
-                       : launch_norm_grad_rows<T, 1>(a, st, &wide);
+  const int rc = packs   ? launch_norm_grad_rows<T, kVec, false>(a, st, &wide)
+                 : shift ? launch_norm_grad_rows<T, kVec, true>(a, st, &wide)
+                         : launch_norm_grad_rows<T, 1, false>(a, st, &wide);
   if (!wide) return rc;
   a.n_part = static_cast<int>(std::min<int64_t>(a.rows, kNormParts));
   norm_grad_wide_kernel<T><<<a.n_part, 256, 0, st>>>(a);

@@ -174,6 +174,43 @@ def test_gradients(T, K, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("K,gap", [(1001, 8), (1001, 5), (67, 16), (2047, 8), (5003, 16), (9, 8)])
+def test_odd_rows_keep_to_themselves(K, gap, dt):
+    """Widths that no vector divides, alone and as the middle of wider rows:
+    what stands before, behind and in the rows beside reaches no row."""
+    T = 83
+    x, w, r = make(T, K, dt, dt, True, seed=K)
+    dy, dh = make(T, K, dt, dt, True, seed=K + 1)[::2]
+
+    def wide(t):  # the same rows with NaN between them
+        b = torch.full((T, K + gap), float("nan"), dtype=dt, device=DEV)
+        b[:, :K] = t
+        return b[:, :K]
+
+    def run(x, w, r, dy, dh):
+        leaves = [t.detach().requires_grad_() for t in (x, w, r)]
+        y, h = norm.rms_norm(leaves[0], leaves[1], 1e-6, leaves[2])
+        g = torch.autograd.grad([y, h], leaves, [dy, dh])
+        return [y.detach(), h.detach(), g[0], g[2], *norm.rms_norm_quant_int8(x, w, 1e-6, r)[:2], g[1]]
+
+    check_forward(x, w, r, 1e-6)
+    check_grad(x, w, r, 1e-6, dy, dh)
+    want = run(x, w, r, dy, dh)
+    check_forward(wide(x), w, wide(r), 1e-6)
+    check_grad(wide(x), w, wide(r), 1e-6, wide(dy), wide(dh))
+    if gap % 8 == 0:  # the same kernel, so the same bits
+        got = run(wide(x), w, wide(r), wide(dy), wide(dh))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    bad = torch.arange(T, device=DEV) % 3 == 1
+    for t in (x, r, dy, dh):
+        t[bad] = float("nan")
+        got = run(x, w, r, dy, dh)
+        for a, b in zip(got[:-1], want[:-1]):
+            assert torch.equal(a[~bad], b[~bad])
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     """Directional derivatives of the formula in 64 bits, by central
     differences (error about 1e-9 at this step), against the fp32 gradients."""
