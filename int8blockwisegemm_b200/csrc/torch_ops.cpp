@@ -8,6 +8,7 @@
 
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -74,8 +75,9 @@ i8moe_stream_t stream_of(const Tensor& t) {
   return at::cuda::getCurrentCUDAStream(t.get_device()).stream();
 }
 
+// Past the dispatcher: half a microsecond less per tensor.
 Tensor empty(at::IntArrayRef size, const Tensor& like, at::ScalarType type) {
-  return at::empty(size, like.options().dtype(type).requires_grad(false));
+  return Tensor(at::detail::empty_cuda(size, type, like.device(), std::nullopt));
 }
 
 // A gradient function of these operators runs once: their gradients are no
