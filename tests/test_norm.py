@@ -129,6 +129,17 @@ def test_values_at_the_edges(dt):
         assert q.shape == (T, K) and s.shape == (T,)
 
 
+@pytest.mark.gpu
+def test_int8_of_the_largest_values():
+    """Rows up to the last binade of fp32: q is 127 where |y| is largest."""
+    x, _, _ = make(6, 256, torch.float32, torch.float32, False, seed=8)
+    w = torch.full((256,), 5e37, device=DEV)
+    for s in (1.0, 2.0 ** -20, 2.0 ** -120):
+        check_forward(x, w * s, None, 1e-6)
+    q, scale, _, _ = norm.rms_norm_quant_int8(x, w)
+    assert float(scale.max()) * 127 > 2.0 ** 126 and (q.abs().amax(1) == 127).all()
+
+
 def check_grad(x, w, r, eps, dy, dh):
     dt, K = x.dtype, x.size(-1)
     leaves = [t.detach().clone().requires_grad_() for t in ([x, w] if r is None else [x, w, r])]
