@@ -368,8 +368,9 @@ int i8moe_quantize_weights_int4(const void* w, int dtype, int64_t n_expert, int6
  * or permuted_idx[r] / topk when that is non-NULL.  out [n_rows, n] = y; with
  * silu != 0 out [n_rows, n / 2] = silu(y[:, :n/2]) * y[:, n/2:].  Sums are
  * fp32, rounded once at the end.  Rows outside every expert keep what they
- * held.  x bf16 / fp16 with rows x_stride elements apart (16-byte aligned),
- * out and scale of x's dtype. */
+ * held.  Offsets that are out of order or leave the rows set the error word,
+ * and nothing is written.  x bf16 / fp16 with rows x_stride elements apart
+ * (16-byte aligned), out and scale of x's dtype. */
 int i8moe_int4_grouped_mv(const void* x, int64_t x_stride, int64_t x_rows, int dtype,
                           const int32_t* permuted_idx, int64_t topk, const uint8_t* w_packed,
                           const void* w_scale, int64_t group_size, const int32_t* expert_offsets,

@@ -50,15 +50,13 @@ struct MvArgs {
   void* out;  // [rows, N] or [rows, N / 2]
 };
 
-// Rows of expert e, clipped to the output: empty (and the error bit) when the
-// offsets are out of order.
-__device__ __forceinline__ void expert_rows(const MvArgs& a, int e, int64_t* r0, int64_t* r1) {
-  *r0 = __ldg(a.eo + e);
-  *r1 = __ldg(a.eo + e + 1);
-  if (*r0 < 0 || *r1 < *r0 || *r1 > a.rows) {
-    atomicOr(&g_err_int4, kErrBadProblem);
-    *r1 = *r0;
-  }
+// Rows of expert e, or -1 (and the error bit) when the offsets are out of order
+// or leave the output.
+__device__ __forceinline__ int64_t expert_rows(const MvArgs& a, int e) {
+  const int64_t r0 = __ldg(a.eo + e), r1 = __ldg(a.eo + e + 1);
+  if (r0 >= 0 && r0 <= r1 && r1 <= a.rows) return r1 - r0;
+  atomicOr(&g_err_int4, kErrBadProblem);
+  return -1;
 }
 
 __device__ __forceinline__ int64_t source_row(const MvArgs& a, int64_t r) {
@@ -194,7 +192,7 @@ constexpr int kMvMaxExperts = 2048;
 // at the end.
 //
 // Bound by instruction issue beside memory: 128 tokens' first product (256
-// experts, K 2048, 2 x 512 columns, 277 MB) takes 62 us, 4.5 TB/s; the loads
+// experts, K 2048, 2 x 512 columns, 277 MB) takes 61 us, 4.5 TB/s; the loads
 // alone take 49 us, and without them 60.
 //
 // A warp's weights (16 kTiles rows x 128 columns a step) come through its own
@@ -219,15 +217,17 @@ __global__ void __launch_bounds__(kMvThreads, 1) mv_mma_kernel(MvArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, q = lane & 3;
 
-  // s_first[e]: expert e's first chunk
+  // s_first[e]: expert e's first chunk.  Offsets that are not in order are
+  // refused as a whole, so that the chunks are as many as the launch allowed for.
   {
+    bool bad = false;
     const int per = (a.n_expert + kMvThreads - 1) / kMvThreads;
     const int e0 = tid * per;
     int own = 0;
     for (int e = e0; e < min(a.n_expert, e0 + per); ++e) {
-      int64_t r0, r1;
-      expert_rows(a, e, &r0, &r1);
-      const int n = static_cast<int>((r1 - r0 + kMvChunk - 1) / kMvChunk);
+      const int64_t rows = expert_rows(a, e);
+      bad |= rows < 0;
+      const int n = rows < 0 ? 0 : static_cast<int>((rows + kMvChunk - 1) / kMvChunk);
       s_first[e + 1] = n;
       own += n;
     }
@@ -246,20 +246,26 @@ __global__ void __launch_bounds__(kMvThreads, 1) mv_mma_kernel(MvArgs a) {
       s_first[e + 1] = at;
     }
     if (tid == 0) s_first[0] = 0;
-    __syncthreads();
+    if (__syncthreads_or(bad)) return;
   }
 
   const int n_out = kSilu ? a.n / 2 : a.n;
   const int blocks = (n_out + kCols - 1) / kCols;
-  const int64_t total = static_cast<int64_t>(s_first[a.n_expert]) * blocks;
-  const int64_t u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
+  // shares of the units, and of their steps, as equal as can be; in 32 bits,
+  // since 64-bit divisions took 1.5 of one token's 10 us
+  auto split = [](uint32_t n, uint32_t parts, uint32_t i) {
+    const uint32_t each = n / parts;
+    return static_cast<int>(each * i + min(i, n - each * parts));
+  };
+  const int total = s_first[a.n_expert] * blocks;
+  const int u0 = split(total, gridDim.x, blockIdx.x), u1 = split(total, gridDim.x, blockIdx.x + 1);
   if (u0 == u1) return;
   const int steps = (a.k + kMvStep - 1) / kMvStep;
   const int row_bytes = a.k / 2;
   // this warp's steps of the CTA's
-  const int64_t all = (u1 - u0) * steps;
-  auto share = [&](int w) { return all * w / kMvWarps; };
-  const int64_t i0 = share(warp), i1 = share(warp + 1);
+  const int all = (u1 - u0) * steps;
+  auto share = [&](int w) { return split(all, kMvWarps, w); };
+  const int i0 = share(warp), i1 = share(warp + 1);
 
   // A unit: the rows of a chunk and a block of columns
   struct Unit {
@@ -446,15 +452,15 @@ __global__ void __launch_bounds__(kMvThreads, 1) mv_mma_kernel(MvArgs a) {
   clear();
   clear_x();
   if (i0 < i1) {
-    const int64_t u = u0 + i0 / steps;
-    step = from = static_cast<int>(i0 % steps);
-    cur.chunk = static_cast<int>(u / blocks);
-    cur.block = static_cast<int>(u - static_cast<int64_t>(cur.chunk) * blocks);
+    const int u = u0 + i0 / steps;
+    step = from = i0 % steps;
+    cur.chunk = u / blocks;
+    cur.block = u - cur.chunk * blocks;
     find_chunk(cur);
     Unit ahead = cur;
     find_weights(ahead);
     int st_ahead = step;
-    int64_t i_ahead = i0;
+    int i_ahead = i0;
     auto copy_next = [&](int slot) {
       if (i_ahead < i1) {
         copy_weights(st_ahead, slot);
@@ -474,7 +480,7 @@ __global__ void __launch_bounds__(kMvThreads, 1) mv_mma_kernel(MvArgs a) {
     load_x(step);
 
     int slot = 0;
-    for (int64_t left = i1 - i0; left > 0; --left) {
+    for (int left = i1 - i0; left > 0; --left) {
       // x in the weights' pairing: b[word][j] = (x[j], x[j + 4])
       uint32_t b[4][4];
 #pragma unroll
@@ -566,7 +572,7 @@ __global__ void __launch_bounds__(kMvThreads, 1) mv_mma_kernel(MvArgs a) {
   __syncthreads();
   if (!open) return;
   // the warps after this one that have steps of its last unit
-  const int64_t end = i1 + (steps - step);
+  const int end = i1 + (steps - step);
   for (int v = warp + 1; v < kMvWarps && share(v) < end; ++v) {
     if (share(v) == share(v + 1)) continue;
 #pragma unroll
@@ -586,6 +592,9 @@ int launch_mv_kernel(const MvArgs& a, int64_t units, cudaStream_t st) {
   const int smem = kMvWarps * kMvSlots * kTiles * kMvTileBytes +
                    (kMvWarps - 1) * kTiles * 32 * static_cast<int>(sizeof(float4)) +
                    (a.n_expert + 1) * static_cast<int>(sizeof(int));
+  const int64_t sms = num_sms(current_device()), steps = (a.k + kMvStep - 1) / kMvStep;
+  I8_REQUIRE(units < (int64_t(1) << 31) && (units / sms + 1) * steps < (int64_t(1) << 31),
+             "int4_grouped_mv: too many rows for one call");
   auto kernel = mv_mma_kernel<T, G, kTiles, kSilu>;
   constexpr int kMost = kMvWarps * kMvSlots * kTiles * kMvTileBytes +
                         (kMvWarps - 1) * kTiles * 32 * 16 + 4 * (kMvMaxExperts + 1);
@@ -595,8 +604,7 @@ int launch_mv_kernel(const MvArgs& a, int64_t units, cudaStream_t st) {
     I8_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
-  const unsigned grid =
-      static_cast<unsigned>(std::min<int64_t>(units, num_sms(current_device())));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, sms));
   kernel<<<grid, kMvThreads, smem, st>>>(a);
   return check_launch("int4_grouped_mv");
 }

@@ -273,6 +273,7 @@ def test_bad_indices_are_reported():
         out = torch.full((3, N), 5.0, dtype=torch.bfloat16, device=DEV)
         int4.int4_grouped_mv(x, packed, scale, torch.tensor(eo, dtype=torch.int32, device=DEV), G, out=out)
         assert _lib.device_error(0, clear=True) == 1 << 4, eo
+        assert (out == 5).all()
 
 
 @pytest.mark.gpu
