@@ -172,14 +172,14 @@ struct alignas(sizeof(T) * kCount) ScalePack {
   T v[kCount];
 };
 
-// One CTA an SM: 12 warps of 158 registers take 62 us for the decode case's
+// One CTA an SM: 12 warps of 160 registers take 62 us for the decode case's
 // first product, 16 of 128 (with spills) 70, 8 of 172 72.
 constexpr int kMvThreads = 384;
 constexpr int kMvWarps = kMvThreads / 32;
-constexpr int kMvChunk = 8;          // rows of a chunk, one n8 tile: two cost 88 us in that case,
-                                     // and gain 9 % only from 16 rows an expert on
+constexpr int kMvChunk = 8;          // rows of a chunk, one n8 tile: two take 103 us in that case,
+                                     // and 49 instead of 43 with 16 rows an expert
 constexpr int kMvStep = 128;         // columns of a step
-constexpr int kMvSlots = 2;          // steps of weights in flight; more would leave L1 too small
+constexpr int kMvSlots = 2;          // steps of weights in flight: three take 64 us
 constexpr int kMvTileBytes = 16 * kMvStep / 2;
 constexpr int kMvMaxExperts = 2048;
 
@@ -617,8 +617,8 @@ int launch_mv_group(const MvArgs& a, int64_t units, cudaStream_t st) {
 }
 
 // Units of four tiles, or of two where the former leave SMs without work (one
-// row of 4096 x 4096: 10.3 us instead of 12.3; with work for all SMs twice the
-// loads of x cost more, 16.5 instead of 14.5 us for 4 tokens of the decode
+// row of 4096 x 4096: 8.3 us instead of 10.4; with work for all SMs twice the
+// loads of x cost more, 16.4 instead of 14.5 us for 4 tokens of the decode
 // case).
 template <typename T, bool kSilu>
 int launch_mv(const MvArgs& a, cudaStream_t st) {

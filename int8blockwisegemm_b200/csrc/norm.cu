@@ -220,9 +220,9 @@ __device__ __forceinline__ void store_pack(T* row, int i, int k, const Pack<T, k
 // scale follows, rstd being one factor of the row) are reduced together.  kVec
 // is 16 bytes' worth when width, strides and pointers allow it, with kShift or
 // without, else 1.
-// Bound by memory: 8192 x 2048 bf16 with a residual takes 26 us, 5.2 TB/s of
-// the 6.6 that a copy has; with two packs a thread 27, with four 30, with CTAs
-// that stay and load the next row ahead 31.
+// Bound by memory: 8192 x 2048 bf16 with a residual takes 24 us, 5.6 TB/s of
+// the 6.6 that a copy has; two packs a thread take 1 us more, four 4, and CTAs
+// that stay and load the next row ahead 4.
 template <typename T, int kVec, int kPer, bool kShift, bool kQuant>
 __global__ void __launch_bounds__(1024) norm_row_kernel(NormArgs a) {
   using P = Pack<T, kVec>;
