@@ -222,6 +222,28 @@ def test_odd_rows_keep_to_themselves(K, gap, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_one_tensor_off_the_grid(dt):
+    """Each tensor alone where no vector reaches it, or with a stride of its own."""
+    T, K = 70, 200
+    x, w, r = make(T, K + 8, dt, dt, True, seed=2)
+    dy, dh = make(T, K + 8, dt, dt, True, seed=3)[::2]
+    on = dict(x=x[:, :K], w=w[:K], r=r[:, :K], dy=dy[:, :K], dh=dh[:, :K])
+    for name, t in dict(x=x, r=r, dy=dy, dh=dh).items():
+        args = {**on, name: t[:, 1:K + 1]}
+        check_grad(args["x"], args["w"], args["r"], 1e-6, args["dy"], args["dh"])
+        odd = torch.cat([t, t[:, :3]], 1)[:, :K]  # rows K + 11 apart
+        args = {**on, name: odd}
+        check_grad(args["x"], args["w"], args["r"], 1e-6, args["dy"], args["dh"])
+        if name in "xr":
+            check_forward(args["x"], args["w"], args["r"], 1e-6)
+    for k in (K, K - 1):
+        check_forward(x[:, :k].contiguous(), w[1:k + 1], r[:, :k].contiguous(), 1e-6)
+        check_grad(x[:, :k].contiguous(), w[3:k + 3], r[:, :k].contiguous(), 1e-6,
+                   dy[:, :k].contiguous(), dh[:, :k].contiguous())
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     """Directional derivatives of the formula in 64 bits, by central
     differences (error about 1e-9 at this step), against the fp32 gradients."""
