@@ -17,6 +17,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "norm_index.cuh"
 
 namespace i8moe {
 namespace {
@@ -78,7 +79,7 @@ __device__ __forceinline__ void load_weight(const void* w, int dtype, int i, flo
   }
 }
 
-// The same one by one, 0 outside of the row.
+// The same one by one, 0 outside of the row, of k >= 1 elements.
 template <int kVec, typename W>
 __device__ __forceinline__ void load_elements(const W* w, int i, int k, float* out) {
   if (i >= 0 && i + kVec <= k) {
@@ -88,7 +89,7 @@ __device__ __forceinline__ void load_elements(const W* w, int i, int k, float* o
   } else {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
-      out[e] = Num<W>::to_f(w[min(max(i + e, 0), k - 1)]);
+      out[e] = Num<W>::to_f(w[nearest_element(i + e, k)]);
       if (i + e < 0 || i + e >= k) out[e] = 0.f;
     }
   }
@@ -182,18 +183,6 @@ struct alignas(sizeof(T) * kVec) Pack {
   T v[kVec];
 };
 
-// Rows whose width no pack divides (kShift in the kernels): where every tensor
-// starts on 16 bytes and its stride leaves the same remainder as the width, row
-// r begins shift_of(r, k) elements behind a 16-byte boundary in all of them, so
-// that packs counted from that boundary are aligned everywhere; the first and
-// the last one reach over the row's ends.  Only the weight is off by the shift.
-// 4096 x 2047 bf16 with a residual: 23 us instead of 31 element by element,
-// with its gradients 55 instead of 74.
-template <int kVec>
-__device__ __forceinline__ int shift_of(int64_t r, int k) {
-  return static_cast<int>((static_cast<uint32_t>(r) * static_cast<uint32_t>(k)) % kVec);
-}
-
 // Zeros the elements outside of the row.
 template <typename T, int kVec>
 __device__ __forceinline__ void trim(Pack<T, kVec>& v, int i, int k) {
@@ -228,9 +217,9 @@ __global__ void __launch_bounds__(1024) norm_row_kernel(NormArgs a) {
   using P = Pack<T, kVec>;
   __shared__ float s_sum[32], s_max[32];
   const int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-  const int k = r < a.rows ? a.k : 0;
   const int tid = threadIdx.x, stride = blockDim.x * kVec;
-  const int shift = kShift ? shift_of<kVec>(r, a.k) : 0, first = tid * kVec - shift;
+  const RowPart part = row_part<kVec, kShift>(r, a.rows, a.k, tid);
+  const int k = part.k, first = part.first, shift = tid * kVec - first;
   const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
   const T* res = static_cast<const T*>(a.residual) + r * a.residual_stride;
   P xv[kPer], rv[kPer];
@@ -675,17 +664,9 @@ uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 template <int kVec>
 bool same_shift(int k, int64_t stride) { return stride >= k && stride % kVec == k % kVec; }
 
-// Columns that the threads of a row have to cover.
-template <int kVec, bool kShift>
-constexpr int covered(int k) { return k + (kShift ? kVec - 1 : 0); }
-
 template <typename T, int kVec, int kPer, bool kShift>
 void launch_norm_row(const NormArgs& a, cudaStream_t st) {
-  const int need = (covered<kVec, kShift>(a.k) + kVec * kPer - 1) / (kVec * kPer);
-  int x = 1;
-  while (x < 32 && x < need) x *= 2;
-  if (need > 32) x = (need + 31) / 32 * 32;
-  const int y = x <= 32 ? 128 / x : 1;
+  const auto [x, y] = row_block<kVec, kPer, kShift>(a.k);
   auto kernel = a.q ? norm_row_kernel<T, kVec, kPer, kShift, true>
                     : norm_row_kernel<T, kVec, kPer, kShift, false>;
   kernel<<<static_cast<unsigned>((a.rows + y - 1) / y), dim3(x, y), 0, st>>>(a);
