@@ -156,7 +156,9 @@ int i8moe_moe_permute(const void* input, int dtype, int64_t n_hidden, const int3
  * finalizeMoeRoutingKernel moe_permute_unpermute_kernel.inl:132-206):
  *   out[t] = dtype( sum_j fma(topk_weights[t,j], permuted[inv[t,j]], acc) )
  * skipping rows >= expert_first_token_offset[n_local_expert] when that
- * pointer is non-NULL. */
+ * pointer is non-NULL, and negative indices.  permuted_hidden may be NULL where
+ * there are no rows (a rank without tokens): out is zeros then.  Otherwise its
+ * first row may be read for slots that are skipped. */
 int i8moe_moe_unpermute(const void* permuted_hidden, int dtype, const float* topk_weights,
                         const int32_t* inv_permuted_idx,
                         const int64_t* expert_first_token_offset, int64_t n_local_expert,

@@ -455,7 +455,9 @@ __global__ void expand_rows(const uint4* __restrict__ in, uint4* __restrict__ ou
 // j order (finalizeMoeRoutingKernel, .inl:132-188).  One token per CTA, four of
 // its rows in flight: loads without a condition (rows that do not count are
 // replaced by the first one, whose values are dropped), so that the compiler
-// issues them together.
+// issues them together.  There is a first row, then: the entry point launches
+// this for tensors that have rows (a choice of another address in the kernel
+// takes 3 us more of 57).
 template <typename T>
 __global__ void __launch_bounds__(256, 6) unpermute_kernel(const T* __restrict__ x,
                                                            const float* __restrict__ w,
@@ -862,9 +864,13 @@ int i8moe_moe_unpermute(const void* permuted_hidden, int dtype, const float* top
                      16 == 0,
                  "moe_unpermute: tensors must be 16-byte aligned");
   if (n_token == 0 || n_hidden == 0) return I8MOE_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (permuted_hidden == nullptr) {  // no rows: empty sums
+    I8_CUDA(cudaMemsetAsync(out, 0, static_cast<size_t>(n_token) * row_bytes, st));
+    return I8MOE_OK;
+  }
   const int vpr = static_cast<int>(row_bytes / 16);
   const int threads = std::min(256, std::max(32, ((vpr + 31) / 32) * 32));
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int nl = static_cast<int>(n_local_expert);
   const int k = static_cast<int>(topk);
   const dim3 grid(static_cast<unsigned>(n_token));
