@@ -156,14 +156,23 @@ int i8moe_moe_permute(const void* input, int dtype, int64_t n_hidden, const int3
  * finalizeMoeRoutingKernel moe_permute_unpermute_kernel.inl:132-206):
  *   out[t] = dtype( sum_j fma(topk_weights[t,j], permuted[inv[t,j]], acc) )
  * skipping rows >= expert_first_token_offset[n_local_expert] when that
- * pointer is non-NULL, and negative indices.  permuted_hidden may be NULL where
- * there are no rows (a rank without tokens): out is zeros then.  Otherwise its
- * first row may be read for slots that are skipped. */
+ * pointer is non-NULL, and negative indices.  Rows that are skipped are not read,
+ * and permuted_hidden may be NULL where there are none (a rank without tokens).
+ * Indices that count have to lie in permuted_hidden, which may have more rows
+ * than n_token * topk. */
 int i8moe_moe_unpermute(const void* permuted_hidden, int dtype, const float* topk_weights,
                         const int32_t* inv_permuted_idx,
                         const int64_t* expert_first_token_offset, int64_t n_local_expert,
                         int64_t n_token, int64_t topk, int64_t n_hidden, void* out,
                         i8moe_stream_t stream);
+
+/* The same for a permuted_hidden of n_rows rows: indices that count and are
+ * not below n_rows are skipped and set the error word (bit 5). */
+int i8moe_moe_unpermute_rows(const void* permuted_hidden, int64_t n_rows, int dtype,
+                             const float* topk_weights, const int32_t* inv_permuted_idx,
+                             const int64_t* expert_first_token_offset, int64_t n_local_expert,
+                             int64_t n_token, int64_t topk, int64_t n_hidden, void* out,
+                             i8moe_stream_t stream);
 
 /* Rows to the experts and back in training (no reference counterpart).  The
  * maps and offsets are those of i8moe_moe_permute_metadata; sorted rows past

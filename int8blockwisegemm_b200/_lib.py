@@ -52,6 +52,7 @@ PROTOTYPES = {
     "i8moe_moe_permute": (I32, [P, I32, I64, P, P, P, I64, I64, I64, I64, P, P, P, P, P, c_size_t,
                                 P]),
     "i8moe_moe_unpermute": (I32, [P, I32, P, P, P, I64, I64, I64, I64, P, P]),
+    "i8moe_moe_unpermute_rows": (I32, [P, I64, I32, P, P, P, I64, I64, I64, I64, P, P]),
     "i8moe_moe_scatter_rows": (I32, [P, I32, P, P, I64, I64, I64, I64, P, P]),
     "i8moe_moe_permute_backward": (I32, [P, I32, P, P, I64, I64, I64, I64, P, P]),
     "i8moe_moe_unpermute_backward": (I32, [P, P, I32, P, P, P, I64, I64, I64, I64, P, P, P]),

@@ -314,9 +314,11 @@ def _unpermute(x, w, inv, eft, topk, out):
     _check(x.dtype in _DT, "moe_unpermute: unsupported dtype")
     n_token, n_hidden = out.shape
     n_local = eft.size(0) - 1 if eft is not None else 0
+    rows = x.numel() // n_hidden if n_hidden else 0
     with torch.cuda.device(out.device):
-        call("i8moe_moe_unpermute", x.data_ptr(), _DT[x.dtype], w.data_ptr(), inv.data_ptr(),
-             _ptr(eft), n_local, n_token, topk, n_hidden, out.data_ptr(), _stream(out))
+        call("i8moe_moe_unpermute_rows", x.data_ptr(), rows, _DT[x.dtype], w.data_ptr(),
+             inv.data_ptr(), _ptr(eft), n_local, n_token, topk, n_hidden, out.data_ptr(),
+             _stream(out))
 
 
 def _silu_and_mul(out, inp):

@@ -76,6 +76,19 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// 16 bytes of global memory that this kernel does not write and reads once, or
+// zeros where `on` is negative: no access then, and no branch either, so that
+// several such loads are in flight together.
+__device__ __forceinline__ uint4 load_if(int on, const uint4* p) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  asm volatile(
+      "{\n.reg .pred on;\nsetp.ge.s32 on, %4, 0;\n"
+      "@on ld.global.nc.L1::evict_first.v4.u32 {%0,%1,%2,%3}, [%5];\n}"
+      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+      : "r"(on), "l"(p));
+  return v;
+}
+
 // ---------------------------------------------------------------------------
 // mbarrier
 // ---------------------------------------------------------------------------

@@ -88,12 +88,10 @@ __global__ void __launch_bounds__(256) scatter_rows_kernel(RowArgs a, const uint
   }
 }
 
-// One token per CTA, four of its rows in flight: loads without a condition
-// (rows that do not count are replaced by the first one, whose values are
-// dropped), so that the compiler issues them together.  Where no row counts, the
-// token's own output row stands in for the first one.  Bound by memory: 8192 x
-// 2048 bf16, top 8 (302 MB) takes 47.5 us, 6.4 of the 6.6 TB/s of a copy; with
-// conditional loads 63, with eight rows and registers for four CTAs an SM 56.
+// One token per CTA, four of its rows in flight by predicated loads; rows that do
+// not count are not read.  Bound by memory: 8192 x 2048 bf16, top 8 (302 MB) takes
+// 43 us, 7.0 TB/s (a copy, which writes half of its bytes, has 6.6); with branches
+// around the loads 63, without the loads' evict-first hint 48.
 template <typename T>
 __global__ void __launch_bounds__(256, 6) gather_sum_kernel(RowArgs a,
                                                             const uint4* __restrict__ rows,
@@ -101,7 +99,6 @@ __global__ void __launch_bounds__(256, 6) gather_sum_kernel(RowArgs a,
   constexpr int EPV = 16 / sizeof(T), kSlots = 4;
   const int valid = valid_rows(a);
   const int64_t t = blockIdx.x;
-  const uint4* first = valid > 0 ? rows : out + t * a.vpr;
   for (int v = threadIdx.x; v < a.vpr; v += blockDim.x) {
     float acc[EPV];
 #pragma unroll
@@ -113,7 +110,7 @@ __global__ void __launch_bounds__(256, 6) gather_sum_kernel(RowArgs a,
 #pragma unroll
       for (int j = 0; j < kSlots; ++j) {
         if (d[j] >= valid) d[j] = -1;
-        raw[j] = __ldg(vec(first, a, d[j] < 0 ? 0 : d[j], v));
+        raw[j] = load_if(d[j], vec(rows, a, d[j], v));
       }
 #pragma unroll
       for (int j = 0; j < kSlots; ++j) {

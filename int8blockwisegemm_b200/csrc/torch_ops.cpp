@@ -32,7 +32,7 @@ struct Library {
   decltype(&i8moe_route_workspace_size) route_workspace_size;
   decltype(&i8moe_moe_permute_metadata) moe_permute_metadata;
   decltype(&i8moe_moe_scatter_rows) moe_scatter_rows;
-  decltype(&i8moe_moe_unpermute) moe_unpermute;
+  decltype(&i8moe_moe_unpermute_rows) moe_unpermute_rows;
   decltype(&i8moe_moe_permute_backward) moe_permute_backward;
   decltype(&i8moe_moe_unpermute_backward) moe_unpermute_backward;
   decltype(&i8moe_rms_norm) rms_norm;
@@ -48,7 +48,7 @@ void bind(const std::unordered_map<std::string, uintptr_t>& address) {
   I8_BIND(route_workspace_size);
   I8_BIND(moe_permute_metadata);
   I8_BIND(moe_scatter_rows);
-  I8_BIND(moe_unpermute);
+  I8_BIND(moe_unpermute_rows);
   I8_BIND(moe_permute_backward);
   I8_BIND(moe_unpermute_backward);
   I8_BIND(rms_norm);
@@ -372,10 +372,10 @@ struct ReturnRows : torch::autograd::Function<ReturnRows> {
                         const Tensor& inv, const optional<Tensor>& eft) {
     const c10::cuda::CUDAGuard guard(rows.device());
     Tensor out = empty({weights.size(0), rows.size(1)}, rows, rows.scalar_type());
-    check(lib.moe_unpermute(rows.data_ptr(), type_of(rows),
-                            static_cast<const float*>(weights.data_ptr()), ints(inv), offsets(eft),
-                            experts(eft), weights.size(0), weights.size(1), rows.size(1),
-                            out.data_ptr(), stream_of(rows)),
+    check(lib.moe_unpermute_rows(rows.data_ptr(), rows.size(0), type_of(rows),
+                                 static_cast<const float*>(weights.data_ptr()), ints(inv),
+                                 offsets(eft), experts(eft), weights.size(0), weights.size(1),
+                                 rows.size(1), out.data_ptr(), stream_of(rows)),
           "moe_unpermute_train");
     ctx->save_for_backward({rows, weights, inv, eft ? *eft : Tensor()});
     ctx->set_materialize_grads(false);

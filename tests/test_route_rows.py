@@ -69,3 +69,60 @@ def test_rows_trimmed_to_the_local_ones(n, dt):
     all_rows[:n] = x.float()
     want = (all_rows[inv.long()].view(T, topk, K) * w[..., None]).sum(1)
     assert torch.equal(out, want.to(dt))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_a_map_into_padded_rows(dt):
+    """A caller's own layout with gaps between the experts' rows: more rows
+    than slots, and every index that the tensor has counts."""
+    T, topk, K, rows = 30, 2, 64, 150
+    g = torch.Generator().manual_seed(0)
+    inv = torch.randperm(rows, generator=g)[:T * topk].to(torch.int32).to(DEV)
+    assert int(inv.max()) >= T * topk
+    x, w = integers(rows, K, dt=dt), integers(T, topk, seed=1)
+    want = (x[inv.long()].float().view(T, topk, K) * w[..., None]).sum(1).to(dt)
+    out = torch.empty(T, K, dtype=dt, device=DEV)
+    for eft in (None, torch.tensor([0, 70, rows], device=DEV)):
+        permute.moe_unpermute(out.fill_(7.0), x, w, inv, eft)
+        assert torch.equal(out, want)
+    lib, p = _lib.LIB, ctypes.c_void_p
+    out.fill_(7.0)
+    rc = lib.i8moe_moe_unpermute(p(x.data_ptr()), DTYPES.index(dt), p(w.data_ptr()), p(inv.data_ptr()), None, 0, T,
+                                 topk, K, p(out.data_ptr()), p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0 and torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("train", [False, True])
+def test_indices_outside_of_the_rows_are_reported(train):
+    T, topk, K = 4, 2, 64
+    x, w = integers(T * topk, K), integers(T, topk, seed=1)
+    inv = i32([0, 1, 2, 8, 4, 5, 6, 7])  # 8 is no row
+
+    def run(inv, eft):
+        if train:
+            return permute.moe_unpermute_train(x, w, inv, eft)
+        out = torch.empty(T, K, device=DEV)
+        permute.moe_unpermute(out, x, w, inv, eft)
+        return out
+
+    for eft in (None, torch.tensor([0, 9], device=DEV)):
+        out = run(inv, eft)
+        assert torch.equal(out[1], w[1, 0] * x[2]) and torch.equal(out[0], w[0, 0] * x[0] + w[0, 1] * x[1])
+        assert _lib.device_error(0, clear=True) == 1 << 5
+    run(inv, torch.tensor([0, 8], device=DEV))  # skipped by the offsets, as rows of other ranks are
+    run(i32([0, 1, 2, -1, 4, 5, 6, 7]), None)  # a slot without a row
+    assert _lib.device_error(0) == 0
+
+
+def test_c_argument_errors_before_any_cuda_call():
+    one = ctypes.c_void_p(256)  # never read
+
+    def call(rows=4, dtype=0, topk=2, k=64, T=2):
+        return _lib.LIB.i8moe_moe_unpermute_rows(one, rows, dtype, one, one, None, 0, T, topk, k, one, None)
+
+    for kw, message in [(dict(rows=-1), "n_rows"), (dict(dtype=3), "dtype"), (dict(topk=0), "topk"),
+                        (dict(k=63), "16 bytes"), (dict(T=-1), "n_token")]:
+        assert call(**kw) == -1 and message in _lib.last_error(), kw
+    assert call(T=0) == 0
