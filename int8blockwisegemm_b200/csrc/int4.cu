@@ -411,9 +411,10 @@ __global__ void __launch_bounds__(kMvThreads, 1) mv_mma_kernel(MvArgs a) {
   // acc[i] holds rows 2 q and 2 q + 1, columns g and g + 8 of tile i; a
   // transpose gives each lane one row and two neighbouring columns
   auto store = [&](const Unit& n) {
-    T* out = static_cast<T*>(a.out) + (n.row0 + g) * n_out;
+    constexpr int kOut = kSilu ? kSetTiles : kTiles;
+    uint32_t pair[kOut][2];
 #pragma unroll
-    for (int i = 0; i < (kSilu ? kSetTiles : kTiles); ++i)
+    for (int i = 0; i < kOut; ++i)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         __align__(4) T v[2];
@@ -423,17 +424,23 @@ __global__ void __launch_bounds__(kMvThreads, 1) mv_mma_kernel(MvArgs a) {
           v[j] = Num<T>::from_f(
               kSilu ? silu_mul(y, acc[kSilu ? i + kSetTiles : i][half * 2 + j]) : y);
         }
-        uint32_t pair = *reinterpret_cast<const uint32_t*>(v);
-        asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(pair));
+        // volatile: all lanes have to take part, also those that store nothing
+        asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;"
+                     : "=r"(pair[i][half]) : "r"(*reinterpret_cast<const uint32_t*>(v)));
+      }
+    if (g >= n.rows) return;
+    T* out = static_cast<T*>(a.out) + (n.row0 + g) * n_out;
+#pragma unroll
+    for (int i = 0; i < kOut; ++i)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
         const int col = n.block * kCols + i * 16 + half * 8 + 2 * q;
-        if (g < n.rows) {
-          const T* p = reinterpret_cast<const T*>(&pair);
-          if (n_out % 2 == 0) {
-            if (col < n_out) *reinterpret_cast<uint32_t*>(out + col) = pair;
-          } else {
-            if (col < n_out) out[col] = p[0];
-            if (col + 1 < n_out) out[col + 1] = p[1];
-          }
+        const T* p = reinterpret_cast<const T*>(&pair[i][half]);
+        if (n_out % 2 == 0) {
+          if (col < n_out) *reinterpret_cast<uint32_t*>(out + col) = pair[i][half];
+        } else {
+          if (col < n_out) out[col] = p[0];
+          if (col + 1 < n_out) out[col + 1] = p[1];
         }
       }
   };
