@@ -78,14 +78,12 @@ __device__ __forceinline__ float silu_mul(float gate, float up) {
 // ---------------------------------------------------------------------------
 // Weights are the m16 operand of mma.m16n8k16 and a chunk of an expert's rows
 // (8 per n8 tile) the other one, so that each weight is read and unpacked once
-// for all rows of the chunk.  A nibble u becomes the 16-bit float base + u by
-// one AND-OR; what that is above u - 8 is taken off by starting the sum at
-// -(base + 8) times the sum of x, one more product per step, by a constant,
-// that all columns share (a subtraction per pair of weights took a fifth of the
-// instructions).  Products are exact in the fp32 accumulators, which are scaled
-// per group, so that no weight is rounded.  The sums carry (base + 8) |x| where
-// the result has up to 8 |x|: that takes up to five of their 24 bits, and the
-// result has 8 (bf16) or 11 (fp16).
+// for all rows of the chunk.  A nibble u becomes the 16-bit float u - 8, exactly;
+// products are exact in the fp32 accumulators, which are scaled per group, so
+// that no weight is rounded and nothing but x (u - 8) enters a sum.  (Sums that
+// start at minus the offset's part, in place of an operation per pair of weights,
+// carry the offset times x: a large x under a zero weight then costs the result
+// its last bits, for 62 instead of 65 us in bf16, and 64 instead of 59 in fp16.)
 //
 // A sum over k may take the k's in any order, so each lane loads what lies
 // together: lane (g, q) = (lane / 4, lane % 4) takes rows g and g + 8 of a tile
@@ -102,13 +100,25 @@ struct Mma;
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), \
         "f"(c[3]))
 
-// Pairs of 16-bit floats.  kBase: base, kMask: where it takes a nibble's bits,
-// at(w, p): w with nibbles p and p + 4 there, kMinus: -(base + 8).
+// u - 8 of nibbles p and p + 4, as a pair of 16-bit floats: one AND-OR (a single
+// three-input operation; the compiler made two of it) puts the nibbles into the
+// fraction of a base, and one operation takes base and offset off again.  Both
+// are exact.
+__device__ __forceinline__ uint32_t masked(uint32_t w, uint32_t mask, uint32_t base) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;"  // (a & b) | c
+      : "=r"(r) : "r"(w), "r"(mask), "r"(base));
+  return r;
+}
 template <>
 struct Mma<__nv_bfloat16> {
   // 7 bits of fraction: 128 + u
-  static constexpr uint32_t kBase = 0x43004300u, kMask = 0x000f000fu, kMinus = 0xc308c308u;
-  static __device__ __forceinline__ uint32_t at(uint32_t w, int p) { return w >> (4 * p); }
+  static __device__ __forceinline__ uint32_t weights(uint32_t w, int p) {
+    uint32_t r;
+    asm("sub.rn.bf16x2 %0, %1, %2;"
+        : "=r"(r) : "r"(masked(w >> (4 * p), 0x000f000fu, 0x43004300u)), "r"(0x43084308u));
+    return r;
+  }
   // d = a * b + c
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                              uint32_t a3, uint32_t b0, uint32_t b1,
@@ -119,10 +129,17 @@ struct Mma<__nv_bfloat16> {
 
 template <>
 struct Mma<__half> {
-  // 10 bits of fraction: 16 + u, the nibble in the upper four
-  static constexpr uint32_t kBase = 0x4c004c00u, kMask = 0x03c003c0u, kMinus = 0xce00ce00u;
-  static __device__ __forceinline__ uint32_t at(uint32_t w, int p) {
-    return p < 2 ? w << (6 - 4 * p) : w >> (4 * p - 6);
+  // 10 bits of fraction: 1024 + u, or 1024 + 16 u
+  static __device__ __forceinline__ uint32_t weights(uint32_t w, int p) {
+    uint32_t r;
+    if (p >= 2) w >>= 8;
+    if (p % 2 == 0)
+      asm("sub.rn.f16x2 %0, %1, %2;"
+          : "=r"(r) : "r"(masked(w, 0x000f000fu, 0x64006400u)), "r"(0x64086408u));
+    else
+      asm("fma.rn.f16x2 %0, %1, %2, %3;"  // / 16 - (64 + 8)
+          : "=r"(r) : "r"(masked(w, 0x00f000f0u, 0x64006400u)), "r"(0x2c002c00u), "r"(0xd480d480u));
+    return r;
   }
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                              uint32_t a3, uint32_t b0, uint32_t b1,
@@ -131,17 +148,6 @@ struct Mma<__half> {
   }
 };
 #undef I8_MMA
-
-// base + u of nibbles p and p + 4, as one three-input operation after the
-// shift (the compiler made two of it: 102 against 90 us for the decode case's
-// first product).
-template <typename T>
-__device__ __forceinline__ uint32_t nibble_pair(uint32_t w, int p) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;"  // (a & b) | c
-      : "=r"(r) : "r"(Mma<T>::at(w, p)), "r"(Mma<T>::kMask), "r"(Mma<T>::kBase));
-  return r;
-}
 
 // 16 bytes to shared memory past L1; `bytes` 0 fills with zeros and reads
 // nothing.
@@ -515,16 +521,7 @@ __global__ void __launch_bounds__(kMvThreads, 1) mv_mma_kernel(MvArgs a) {
       copies_wait<kMvSlots - 1>();
       __syncwarp();
       const uint32_t base = slot * kSlotBytes;
-      // the sums' start
       constexpr float zero[4] = {0.f, 0.f, 0.f, 0.f};
-      float start[kGroups][4];
-#pragma unroll
-      for (int gi = 0; gi < kGroups; ++gi)
-#pragma unroll
-        for (int j = 0; j < 2 * kWords; ++j)
-          Mma<T>::mma(start[gi], Mma<T>::kMinus, Mma<T>::kMinus, Mma<T>::kMinus, Mma<T>::kMinus,
-                      b[gi * kWords + j / 2][j % 2 * 2], b[gi * kWords + j / 2][j % 2 * 2 + 1],
-                      j == 0 ? zero : start[gi]);
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {  // tile i: rows 16 (i % kSetTiles) of set i / kSetTiles
         uint32_t w[2][4];
@@ -543,9 +540,9 @@ __global__ void __launch_bounds__(kMvThreads, 1) mv_mma_kernel(MvArgs a) {
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
-              for (int p = 0; p < 4; ++p) f[half][p] = nibble_pair<T>(w[half][wi], p);
+              for (int p = 0; p < 4; ++p) f[half][p] = Mma<T>::weights(w[half][wi], p);
             Mma<T>::mma(part, f[0][0], f[1][0], f[0][1], f[1][1], b[wi][0], b[wi][1],
-                        j == 0 ? start[gi] : part);
+                        j == 0 ? zero : part);
             Mma<T>::mma(part, f[0][2], f[1][2], f[0][3], f[1][3], b[wi][2], b[wi][3], part);
           }
           const int row = i % kSetTiles * 16 + g;

@@ -55,9 +55,8 @@ def int4_grouped_mv(x, w_packed, w_scale, expert_offsets, group_size: int = 128,
     gate rows and then N/2 up rows, and the result is silu(gate) * up.
     Returns ``out`` [rows, N] (N/2 with silu) in x's type, allocated when not
     given; rows outside every expert keep what it held.  Sums are fp32,
-    rounded once.  A group's sum of up to 128 terms carries up to 143 |x|, so
-    that a row with an infinity gives NaN, and bf16 values above 2^113 may.
-    No gradients."""
+    rounded once; a group's sum comes before its scale, of up to 128 terms of
+    up to 8 |x| (bf16 values above 2^117 may leave fp32).  No gradients."""
     return TORCH_OPS.int4_grouped_mv(x, w_packed, w_scale, expert_offsets, group_size, permuted_idx,
                                      topk, silu, out)
 
