@@ -367,7 +367,8 @@ int i8moe_int8_grouped_mm(const int8_t* a, const int8_t* b, void* out, int out_d
  * holds column k of a row in byte k / 2, low half for even k, as q + 8 with q
  * in [-8, 7]; scale [E, N, ceil(K / group_size)] of scale_dtype.  Per group:
  * scale = max|w| / 7 rounded to its type, q = clamp(rint(w / scale), -8, 7)
- * (ties to even) by the rounded scale; a group of zeros has scale 0.
+ * (ties to even) by the rounded scale; a group of zeros has scale 0, one with a
+ * NaN scale NaN and q 0, one whose scale leaves its type scale inf and q 0.
  * group_size 32, 64 or 128; K a multiple of 32. */
 int i8moe_quantize_weights_int4(const void* w, int dtype, int64_t n_expert, int64_t n, int64_t k,
                                 int64_t group_size, uint8_t* packed, void* scale, int scale_dtype,

@@ -76,6 +76,14 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// The larger one, NaN if either is: a maximum over values shows that one of
+// them is not a number.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // 16 bytes of global memory that this kernel does not write and reads once, or
 // zeros where `on` is negative: no access then, and no branch either, so that
 // several such loads are in flight together.

@@ -636,7 +636,9 @@ int launch_mv(const MvArgs& a, cudaStream_t st) {
 // One warp per group: scale = max|w| / 7 rounded to the scale's type, and
 // u = clamp(rint(w / scale), -8, 7) + 8 by that rounded scale, so that its
 // rounding shifts no weight twice.  A group of zeros (or one whose scale
-// rounds to zero) gets scale 0 and u = 8.
+// rounds to zero) gets scale 0 and u = 8; one with a NaN scale NaN, one with an
+// infinity (or whose scale leaves its type) scale inf, and u = 8 both, so that
+// what is wrong with a weight reaches the products as NaN.
 template <typename T, typename S>
 __global__ void __launch_bounds__(256) quantize_int4_kernel(const T* __restrict__ w, int64_t rows,
                                                             int k, int group, int groups,
@@ -653,9 +655,9 @@ __global__ void __launch_bounds__(256) quantize_int4_kernel(const T* __restrict_
     const int k1 = min(k, k0 + group);
     const T* src = w + row * k;
     float m = 0.f;
-    for (int c = k0 + lane; c < k1; c += 32) m = fmaxf(m, fabsf(Num<T>::to_f(src[c])));
+    for (int c = k0 + lane; c < k1; c += 32) m = max_nan(m, fabsf(Num<T>::to_f(src[c])));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     const S s = Num<S>::from_f(__fdiv_rn(m, 7.f));
     const float sf = Num<S>::to_f(s);
     if (lane == 0) scale[i] = s;

@@ -129,13 +129,6 @@ __device__ __forceinline__ void load_weight_at(const void* w, int dtype, int i, 
   load_elements<kVec>(static_cast<const float*>(w), i, k, out);
 }
 
-// max that keeps NaN, so that a row without a finite norm gets a NaN scale
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 struct Sum {
   static __device__ __forceinline__ float of(float a, float b) { return a + b; }
 };

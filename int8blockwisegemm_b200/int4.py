@@ -29,7 +29,10 @@ def quantize_weights_int4(w: torch.Tensor, group_size: int = 128, scale_dtype=No
     """(packed, scale) of w [E, N, K] (bf16, fp16 or fp32): per group
     scale = max|w| / 7 rounded to ``scale_dtype`` (w's type when omitted) and
     q = clamp(rint(w / scale), -8, 7).  K must be a multiple of 32,
-    group_size 32, 64 or 128; the last group of a row may be shorter."""
+    group_size 32, 64 or 128; the last group of a row may be shorter.  The
+    products take scales of the activations' type: give ``scale_dtype`` for
+    fp32 weights.  A group with a NaN gets scale NaN, one whose scale leaves
+    its type inf; their q is 0 and products by them are NaN.  No gradients."""
     scale_dtype = w.dtype if scale_dtype is None else scale_dtype
     _check(w.is_cuda and w.dim() == 3, "quantize_weights_int4: w must be a CUDA tensor [E, N, K]")
     _check(w.dtype in _DT and scale_dtype in _DT, "quantize_weights_int4: unsupported dtype")

@@ -96,3 +96,34 @@ def test_infinities_and_the_largest_values(dt):
     big = 2.0 ** 115 if dt == torch.bfloat16 else 60000.0
     scale.fill_(2.0 ** -12)
     close_to_formula(torch.full((2, K), big, dtype=dt, device=DEV), packed, scale, G)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wdt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_weights_that_are_not_finite_stay_visible(dt, wdt):
+    """A NaN or an infinity makes its group's scale say so and the products by
+    it NaN; every other group is as it would be without."""
+    E, N, K, G = 2, 6, 256, 64
+    w = (torch.randn(E, N, K, generator=torch.Generator().manual_seed(1)) * 0.05).to(wdt).to(DEV)
+    want_p, want_s = int4.quantize_weights_int4(w, G, dt)
+    bad = {(0, 1, 0): float("nan"), (0, 2, 1): float("inf"), (1, 0, 3): float("-inf"), (1, 5, 2): float("nan")}
+    if wdt == torch.float32 and dt == torch.float16:
+        bad[(1, 3, 1)] = 1e6  # a scale above fp16's range
+    for (e, n, g), v in bad.items():
+        w[e, n, g * G + 7 * g + 3] = v
+    packed, scale = int4.quantize_weights_int4(w, G, dt)
+    for (e, n, g), v in bad.items():
+        s = float(scale[e, n, g])
+        assert s != s if v != v else s == float("inf")
+        assert (packed[e, n, g * G // 2:(g + 1) * G // 2] == 0x88).all()
+        packed[e, n, g * G // 2:(g + 1) * G // 2] = want_p[e, n, g * G // 2:(g + 1) * G // 2]
+    x = rows_of(3, K, dt)
+    got = int4.int4_grouped_mv(x, want_p, scale, offsets([2, 1]), G)
+    rows = torch.zeros(E, N, dtype=torch.bool)
+    for e, n, _ in bad:
+        rows[e, n] = True
+    rows = rows.to(DEV)[torch.tensor([0, 0, 1], device=DEV)]
+    assert torch.equal(packed, want_p) and torch.equal(got.isfinite(), ~rows)
+    whole = int4.int4_grouped_mv(x, *int4.quantize_weights_int4(w, G, dt), offsets([2, 1]), G)
+    assert torch.equal(whole.isnan(), rows)
