@@ -68,9 +68,13 @@ __device__ __forceinline__ int64_t source_row(const MvArgs& a, int64_t r) {
   return -1;
 }
 
-// The quotient's two last bits are below the rounding of the 16-bit result.
+// gate / (1 + exp(-gate)) * up, the exponential of the negative value on either
+// side, so that it cannot overflow and the divisor is in [1, 2]: the fast
+// division, whose two last bits are below the rounding of the 16-bit result,
+// gives 0 for divisors above 2^126.
 __device__ __forceinline__ float silu_mul(float gate, float up) {
-  return __fdividef(gate, 1.f + expf(-gate)) * up;
+  const float e = expf(-fabsf(gate));
+  return __fdividef(gate < 0.f ? gate * e : gate, 1.f + e) * up;
 }
 
 // ---------------------------------------------------------------------------

@@ -127,3 +127,27 @@ def test_weights_that_are_not_finite_stay_visible(dt, wdt):
     assert torch.equal(packed, want_p) and torch.equal(got.isfinite(), ~rows)
     whole = int4.int4_grouped_mv(x, *int4.quantize_weights_int4(w, G, dt), offsets([2, 1]), G)
     assert torch.equal(whole.isnan(), rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_silu_of_very_negative_gates(dt):
+    """A tiny silu times a large factor.  One column per row is not zero, so
+    gates and factors are exact; the exponential, the quotient and the products
+    are off by a few units of 2^-24, and the exponential by a rounding to fp32's
+    smallest values (2^-150)."""
+    gates = [-102.0, -95.0, -89.0, -88.0, -87.5, -87.0, -80.0, -20.0, -1.0, -0.0, 0.5, 20.0, 87.5, 100.0]
+    N, K, G = 16, 64, 32
+    up = 2.0 ** 110 if dt == torch.bfloat16 else 2.0 ** 12
+    packed = torch.full((1, N, K // 2), 0x99, dtype=torch.uint8, device=DEV)  # every q is 1
+    scale = torch.ones(1, N, K // G, dtype=dt, device=DEV)
+    scale[:, N // 2:] = up
+    x = torch.zeros(len(gates), K, dtype=dt, device=DEV)
+    x[:, 5] = torch.tensor(gates, dtype=dt)
+    got = int4.int4_grouped_mv(x, packed, scale, offsets([len(gates)]), G, silu=True).double()
+    g = x[:, 5:6].double().expand(-1, N // 2)
+    y = g * torch.sigmoid(g) * (g * up)
+    tol = y.abs() * (half(dt) + 16 * 2.0 ** -24) + (g * g * up).abs() * 2.0 ** -149 + tiny(dt)
+    over = y.abs() > 1.01 * torch.finfo(dt).max  # fp16's 65504 at the largest gates: rounded to an infinity
+    assert (got[over] == float("inf")).all()
+    assert ((got - y).abs() <= tol)[~over].all(), (got[:, 0], y[:, 0])
