@@ -465,8 +465,8 @@ Tensor int4_grouped_mv(const Tensor& x_in, const Tensor& packed, const Tensor& s
     TORCH_CHECK(topk >= 1, what, ": topk must be positive");
     rows = pidx->size(0);
   }
-  TORCH_CHECK(!(at::GradMode::is_enabled() && x_in.requires_grad()), what,
-              " has no gradient: call it under torch.no_grad()");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && (x_in.requires_grad() || scale.requires_grad())),
+              what, " has no gradient: call it under torch.no_grad()");
   const c10::cuda::CUDAGuard guard(device);
   const int64_t n_out = silu ? N / 2 : N;
   Tensor out;

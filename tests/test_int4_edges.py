@@ -151,3 +151,16 @@ def test_silu_of_very_negative_gates(dt):
     over = y.abs() > 1.01 * torch.finfo(dt).max  # fp16's 65504 at the largest gates: rounded to an infinity
     assert (got[over] == float("inf")).all()
     assert ((got - y).abs() <= tol)[~over].all(), (got[:, 0], y[:, 0])
+
+
+@pytest.mark.gpu
+def test_scales_that_want_a_gradient_are_refused():
+    """As rows that want one are: they would get none."""
+    packed, scale = weights(1, 32, 64, 32, torch.bfloat16)
+    x, eo = rows_of(2, 64, torch.bfloat16), offsets([2])
+    want = int4.int4_grouped_mv(x, packed, scale, eo, 32)
+    scale.requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        int4.int4_grouped_mv(x, packed, scale, eo, 32)
+    with torch.no_grad():
+        assert torch.equal(int4.int4_grouped_mv(x, packed, scale, eo, 32), want)
