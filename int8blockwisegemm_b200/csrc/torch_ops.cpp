@@ -86,6 +86,13 @@ void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once (no create_graph)");
 }
 
+// These operators go past the dispatcher and would leave out the tangents of
+// forward-mode differentiation.
+void no_tangents(const char* what, std::initializer_list<Tensor> inputs) {
+  for (const Tensor& t : inputs)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 // Inside a graph's capture: a leaf whose gradient node lives on in an eager
 // graph brings that graph's stream into the captured backward pass, which ends
 // the process there.  Refused here instead.
@@ -120,6 +127,7 @@ void check_norm(const char* what, const Tensor& x, const Tensor& weight, double 
   TORCH_CHECK(weight.dim() == 1 && weight.size(0) == x.size(-1), what,
               ": weight must have shape [K]");
   TORCH_CHECK(eps >= 0 && eps < 3e38, what, ": eps must be finite and not negative");
+  no_tangents(what, {x, weight, residual ? *residual : Tensor()});
   if (residual) {
     TORCH_CHECK(residual->device() == x.device(), what, ": residual must be on x's device");
     TORCH_CHECK(residual->scalar_type() == x.scalar_type(), what,
@@ -164,6 +172,7 @@ std::tuple<Tensor, optional<Tensor>> rms_norm_backward(
   TORCH_CHECK(rstd.scalar_type() == at::kFloat && rstd.is_contiguous() &&
                   rstd.device() == x.device() && rstd.numel() == x.numel() / x.size(-1),
               what, ": rstd must be float32 [rows] on x's device");
+  no_tangents(what, {dy, rstd, residual_grad ? *residual_grad : Tensor()});
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor xr = rows_of(x), gr = rows_of(dy), w = weight.contiguous();
   Tensor rr, hr;
@@ -291,6 +300,7 @@ Tensor moe_permute_backward(const Tensor& permuted_grad, const Tensor& inv,
   TORCH_CHECK(n_token >= 0 && topk >= 1 && permuted_grad.size(0) == n_token * topk, what,
               ": permuted_grad must have n_token * topk rows");
   check_maps(what, inv, eft, n_token * topk, permuted_grad);
+  no_tangents(what, {permuted_grad});
   const c10::cuda::CUDAGuard guard(permuted_grad.device());
   const Tensor g = aligned(permuted_grad);
   Tensor out = empty({n_token, g.size(1)}, g, g.scalar_type());
@@ -317,6 +327,7 @@ std::tuple<Tensor, Tensor> moe_unpermute_backward(const Tensor& out_grad, const 
                   out_grad.device() == rows.device(),
               what, ": out_grad must be [n_token, hidden] of permuted_hidden_states' dtype");
   check_maps(what, inv, eft, n_token * topk, rows);
+  no_tangents(what, {out_grad, rows, weights});
   const c10::cuda::CUDAGuard guard(rows.device());
   const Tensor g = aligned(out_grad), y = aligned(rows), w = weights.contiguous();
   Tensor dy = empty(y.sizes(), y, y.scalar_type()), dw = empty(w.sizes(), w, at::kFloat);
@@ -410,6 +421,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> moe_permute_train(const Tensor& x, co
                     emap->device() == x.device() && emap->dim() == 1 && emap->size(0) == n_expert,
                 what,
                 ": expert_map must be contiguous int32 [n_expert] on hidden_states' device");
+  no_tangents(what, {x});
   if (at::GradMode::is_enabled()) check_capture(what, {x});
   const variable_list out =
       SortRows::apply(aligned(x), ids.to(at::kInt).contiguous(), emap, n_expert, n_local);
@@ -426,6 +438,7 @@ Tensor moe_unpermute_train(const Tensor& rows, const Tensor& weights, const Tens
               ": permuted_hidden_states must have one row per element of topk_weights "
               "[n_token, topk]");
   check_maps(what, inv, eft, weights.numel(), rows);
+  no_tangents(what, {rows, weights});
   if (at::GradMode::is_enabled()) check_capture(what, {rows, weights});
   return ReturnRows::apply(aligned(rows), weights.to(at::kFloat).contiguous(), inv, eft);
 }
@@ -467,6 +480,7 @@ Tensor int4_grouped_mv(const Tensor& x_in, const Tensor& packed, const Tensor& s
   }
   TORCH_CHECK(!(at::GradMode::is_enabled() && (x_in.requires_grad() || scale.requires_grad())),
               what, " has no gradient: call it under torch.no_grad()");
+  no_tangents(what, {x_in, scale});
   const c10::cuda::CUDAGuard guard(device);
   const int64_t n_out = silu ? N / 2 : N;
   Tensor out;

@@ -19,7 +19,8 @@ passes can be captured into a CUDA graph; drop eager graphs that hold the same
 leaves before capturing a backward pass (a call on such a leaf is refused
 during capture).
 
-Arguments are checked in the compiled binding, which raises RuntimeError.
+Arguments are checked in the compiled binding, which raises RuntimeError, also
+for tensors with a forward-mode tangent: there are no such derivatives.
 """
 
 from __future__ import annotations
