@@ -26,6 +26,7 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libi8moe.so"
 TORCH_OPS = PKG / "_torch_ops.so"
+TORCH_STAMP = BUILD / "torch_ops.stamp"
 INCLUDE = ROOT / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -74,8 +75,12 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
 
     src = CSRC / "torch_ops.cpp"
     header = INCLUDE / "i8moe.h"
+    # what it is built against, beside its sources: another torch or Python has
+    # another ABI
+    against = f"torch {torch.__version__} {torch.version.git_version}, python {sys.version}\n"
     if (not force and TORCH_OPS.exists()
-            and TORCH_OPS.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime)):
+            and TORCH_OPS.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime)
+            and TORCH_STAMP.exists() and TORCH_STAMP.read_text() == against):
         return TORCH_OPS
     cuda = Path(nvcc()).resolve().parent.parent
     includes = [INCLUDE, *cpp_extension.include_paths(), cuda / "include",
@@ -92,6 +97,7 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for {src.name}:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, TORCH_OPS)
+    TORCH_STAMP.write_text(against)
     return TORCH_OPS
 
 

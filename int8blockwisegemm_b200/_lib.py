@@ -102,15 +102,29 @@ def _load():
 LIB = _load()
 
 
+class _NoTorchOps:
+    """In place of the compiled binding where it cannot be loaded: its
+    operators raise, everything bound by ctypes works."""
+
+    def __init__(self, why: str):
+        self._why = why
+
+    def __getattr__(self, name: str):
+        raise RuntimeError(f"{name} is not available: {self._why}\n"
+                           "Build it first:  python int8blockwisegemm_b200/_build.py")
+
+
 def _load_torch_ops():
     """The compiled torch binding of the operators with gradients or single-
     token forms, on the functions of the library that was loaded."""
     try:
         from . import _torch_ops
     except ImportError as exc:
-        raise RuntimeError(
-            "Cannot load _torch_ops.so.\n"
-            "Build it first:  python int8blockwisegemm_b200/_build.py") from exc
+        return _NoTorchOps(f"cannot load _torch_ops.so ({exc})")
+    running = torch.__version__.split("+")[0]
+    if _torch_ops.torch_version != running:
+        return _NoTorchOps(f"_torch_ops.so was built against torch {_torch_ops.torch_version}, "
+                           f"this is {running}")
     _torch_ops.bind({name: ctypes.cast(getattr(LIB, name), c_void_p).value
                      for name in PROTOTYPES})
     return _torch_ops

@@ -5,6 +5,7 @@
 // points are bound by ctypes.  The library's functions are handed over by
 // address, so that INT8_HYBRID_MOE_LIB decides here too.
 #include <torch/extension.h>
+#include <torch/version.h>
 
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -510,6 +511,7 @@ Tensor int4_grouped_mv(const Tensor& x_in, const Tensor& packed, const Tensor& s
 }  // namespace
 
 PYBIND11_MODULE(_torch_ops, m) {
+  m.attr("torch_version") = TORCH_VERSION;
   m.def("bind", &bind);
   m.def("rms_norm", &rms_norm);
   m.def("rms_norm_quant_int8", &rms_norm_quant_int8);
