@@ -75,6 +75,9 @@ def run_int4_moe(output, hidden_states, w1_packed, w1_scale, w2_packed, w2_scale
     a CUDA graph."""
     _check(hidden_states.dim() == 2 and w1_packed.dim() == 3 and w2_packed.dim() == 3,
            "run_int4_moe: hidden_states must be [T, K], the weights [E, rows, columns / 2]")
+    _check(hidden_states.is_cuda and topk_ids.device == hidden_states.device
+           and topk_weights.device == hidden_states.device,
+           "run_int4_moe: hidden_states, topk_ids and topk_weights must be on one CUDA device")
     T, K = hidden_states.shape
     E, two_n, _ = w1_packed.shape
     _check(2 * w1_packed.size(2) == K and w2_packed.shape == (E, K, two_n // 4) and two_n % 4 == 0,

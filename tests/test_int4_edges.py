@@ -164,3 +164,35 @@ def test_scales_that_want_a_gradient_are_refused():
         int4.int4_grouped_mv(x, packed, scale, eo, 32)
     with torch.no_grad():
         assert torch.equal(int4.int4_grouped_mv(x, packed, scale, eo, 32), want)
+
+
+def layer(**change):
+    """A call of the layer with small operands, some of them others."""
+    E, K, N, T, topk = 2, 64, 32, 3, 1
+    d = change.pop("device", DEV)
+    x = torch.zeros(T, K, dtype=torch.bfloat16, device=d)
+    a = dict(output=torch.empty_like(x), hidden_states=x,
+             w1_packed=torch.full((E, 2 * N, K // 2), 0x88, dtype=torch.uint8, device=d),
+             w1_scale=torch.ones(E, 2 * N, 2, dtype=torch.bfloat16, device=d),
+             w2_packed=torch.full((E, K, N // 2), 0x88, dtype=torch.uint8, device=d),
+             w2_scale=torch.ones(E, K, 1, dtype=torch.bfloat16, device=d),
+             topk_ids=torch.zeros(T, topk, dtype=torch.int32, device=d), topk_weights=torch.ones(T, topk, device=d),
+             global_num_experts=E, group_size=32)
+    a.update(change)
+    int4.run_int4_moe(**a)
+    return a["output"]
+
+
+def test_layer_refuses_cpu_tensors():
+    with pytest.raises(RuntimeError, match="one CUDA device"):
+        layer(device="cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["topk_ids", "topk_weights"])
+def test_layer_refuses_routing_on_another_device(name):
+    """Its kernels would read the host's memory."""
+    assert not layer().any()
+    other = dict(topk_ids=torch.zeros(3, 1, dtype=torch.int32), topk_weights=torch.ones(3, 1))[name]
+    with pytest.raises(RuntimeError, match="one CUDA device"):
+        layer(**{name: other})
