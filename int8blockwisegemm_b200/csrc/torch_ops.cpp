@@ -446,6 +446,20 @@ Tensor moe_unpermute_train(const Tensor& rows, const Tensor& weights, const Tens
 
 // ---------------------------------------------------------- 4-bit products
 
+// Whether the contiguous `out` has bytes of a row of x (rows of stride(0) >=
+// size(1) elements); torch's own check gives up on rows with gaps.
+bool rows_meet(const Tensor& x, const Tensor& out) {
+  if (x.numel() == 0 || out.numel() == 0) return false;
+  const int64_t row = x.size(1) * x.element_size(), step = x.stride(0) * x.element_size();
+  const auto start = reinterpret_cast<intptr_t>(x.data_ptr());
+  const int64_t o0 = reinterpret_cast<intptr_t>(out.data_ptr()) - start;
+  const int64_t o1 = o0 + out.numel() * out.element_size();
+  if (o1 <= 0) return false;
+  // the first row that ends behind out's start
+  const int64_t r = o0 < row || step == 0 ? 0 : (o0 - row) / step + 1;
+  return r < x.size(0) && r * step < o1 && r * step + row > o0;
+}
+
 Tensor int4_grouped_mv(const Tensor& x_in, const Tensor& packed, const Tensor& scale,
                        const Tensor& eo, int64_t group, const optional<Tensor>& pidx, int64_t topk,
                        bool silu, const optional<Tensor>& out_in) {
@@ -491,7 +505,7 @@ Tensor int4_grouped_mv(const Tensor& x_in, const Tensor& packed, const Tensor& s
                     out.size(1) == n_out && out.is_contiguous() && out.device() == device,
                 what,
                 ": out must be contiguous [rows, N (N/2 with silu)] of x's dtype on x's device");
-    at::assert_no_overlap(out, x_in);
+    for (const Tensor& t : {x_in, packed, scale, eo, pidx ? *pidx : eo}) at::assert_no_overlap(out, t);
   } else {
     out = empty({rows, n_out}, x_in, x_in.scalar_type());
   }
@@ -500,6 +514,8 @@ Tensor int4_grouped_mv(const Tensor& x_in, const Tensor& packed, const Tensor& s
       (x_in.size(0) < 2 || (x_in.stride(0) % 8 == 0 && x_in.stride(0) >= K)) &&
       reinterpret_cast<uintptr_t>(x_in.data_ptr()) % 16 == 0;
   const Tensor x = in_place ? x_in : aligned(x_in);
+  TORCH_CHECK(!out_in || !rows_meet(x, out), what,
+              ": x and out refer to a single memory location in some elements");
   check(lib.int4_grouped_mv(x.data_ptr(), x.size(0) < 2 ? K : x.stride(0), x.size(0), type_of(x),
                             pidx ? ints(*pidx) : nullptr, topk,
                             static_cast<const uint8_t*>(packed.data_ptr()), scale.data_ptr(), group,

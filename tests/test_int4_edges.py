@@ -196,3 +196,35 @@ def test_layer_refuses_routing_on_another_device(name):
     other = dict(topk_ids=torch.zeros(3, 1, dtype=torch.int32), topk_weights=torch.ones(3, 1))[name]
     with pytest.raises(RuntimeError, match="one CUDA device"):
         layer(**{name: other})
+
+
+@pytest.mark.gpu
+def test_out_may_not_lie_in_what_is_read():
+    """Also where the rows have gaps, in which it may lie."""
+    T, N, K, G, gap = 3, 64, 64, 32, 256
+    packed, scale = weights(1, N, K, G, torch.bfloat16)
+    eo = offsets([T])
+    x = rows_of(T, K, torch.bfloat16)
+    want = int4.int4_grouped_mv(x, packed, scale, eo, G)
+
+    def out_at(start):
+        flat = torch.zeros(T * (K + gap) + T * N, dtype=torch.bfloat16, device=DEV)
+        rows = flat[:T * (K + gap)].view(T, K + gap)[:, :K]
+        rows.copy_(x)
+        return int4.int4_grouped_mv(rows, packed, scale, eo, G, out=flat[start:start + T * N].view(T, N))
+
+    step = K + gap
+    for start in (0, 56, step - 8, step, step + 56, 2 * step - T * N + 8, 2 * step, 2 * step + 56):
+        with pytest.raises(RuntimeError, match="single memory location"):
+            out_at(start)
+    for start in (K, step - T * N, step + K, 2 * step - T * N, 2 * step + K, 3 * step):
+        assert torch.equal(out_at(start), want), start
+    one = torch.zeros(K + N, dtype=torch.bfloat16, device=DEV)  # a single row, whose stride says nothing
+    one[:K] = x[0]
+    row = one[:K].as_strided((1, K), (8, 1))
+    assert torch.equal(int4.int4_grouped_mv(row, packed, scale, offsets([1]), G, out=one[K:].view(1, N)), want[:1])
+    with pytest.raises(RuntimeError, match="single memory location"):
+        int4.int4_grouped_mv(row, packed, scale, offsets([1]), G, out=one[K - 8:K + N - 8].view(1, N))
+    into_scales = scale.view(-1)[:1 * N].view(1, N)
+    with pytest.raises(RuntimeError, match="single memory location"):
+        int4.int4_grouped_mv(x[:1], packed, scale, offsets([1]), G, out=into_scales)
