@@ -158,6 +158,13 @@ __device__ __forceinline__ int8_t to_int8(float y, float inv) {
   return static_cast<int8_t>(__float_as_uint(fmaf(y, inv, 12582912.f)));
 }
 
+// The largest |y| of a row, for its scale: NaN where the sum of squares is not
+// finite (it may leave fp32 where no value does, and every y is 0 then).
+__device__ __forceinline__ float largest_of(float largest, float sum) {
+  const bool finite = sum < __int_as_float(0x7f800000);
+  return finite ? max_nan(largest, 1e-10f) : __int_as_float(0x7fffffff);
+}
+
 // What the int8 values of a row are multiplied by: 127 over its largest |y|.
 // Non-finite rows give 0 and a mask of zeros, which makes their values 0.
 struct Int8Row {
@@ -289,7 +296,7 @@ __global__ void __launch_bounds__(1024) norm_row_kernel(NormArgs a) {
     }
   }
   const float rstd = rsqrtf(fmaf(ss, a.inv_k, a.eps));
-  const float largest = max_nan(m * rstd, 1e-10f);
+  const float largest = largest_of(m * rstd, ss);
   const Int8Row row = int8_row(largest);
   if (tid == 0 && k > 0) {
     if (a.rstd) a.rstd[r] = rstd;
@@ -343,7 +350,7 @@ __global__ void __launch_bounds__(256) norm_wide_kernel(NormArgs a) {
       float m = 0.f;
       for (int i = threadIdx.x; i < a.k; i += blockDim.x)
         m = max_nan(m, fabsf(h_at(i) * rstd * load_any(a.weight, a.weight_dtype, i)));
-      const float largest = max_nan(block_reduce<MaxNan>(m, s_part), 1e-10f);
+      const float largest = largest_of(block_reduce<MaxNan>(m, s_part), ss);
       row = int8_row(largest);
       if (threadIdx.x == 0) a.scale[r] = largest / 127.f;
     }

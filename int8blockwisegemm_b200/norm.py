@@ -30,7 +30,8 @@ from ._lib import TORCH_OPS
 
 def rms_norm(x, weight, eps: float = 1e-6, residual=None):
     """y, or (y, h) with a residual.  Differentiable in x, weight and
-    residual (once); the gradient of weight is summed in a fixed order."""
+    residual (once); the gradient of weight is summed in a fixed order.  Sums
+    of squares are fp32: where one overflows (values of 1e18 and more) y is 0."""
     return TORCH_OPS.rms_norm(x, weight, eps, residual)
 
 
