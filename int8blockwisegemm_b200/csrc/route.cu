@@ -454,9 +454,10 @@ __global__ void expand_rows(const uint4* __restrict__ in, uint4* __restrict__ ou
 // out[t] = dtype(sum_j fma(w[t,j], x[inv[t,j]], acc)), fp32 accumulation in
 // j order (finalizeMoeRoutingKernel, .inl:132-188).  One token per CTA, four of
 // its rows in flight by predicated loads; rows that do not count are not read.
-// Bound by memory: 8192 x 2048 bf16, top 8 (302 MB) takes 44 us, 6.9 TB/s; with
-// branches around the loads 63, without the loads' evict-first hint 49, with six
-// CTAs an SM 46, with eight rows in flight 46.
+// Bound by memory: 8192 x 2048 bf16, top 8 (302 MB) takes 41.7 us, 7.3 TB/s (a
+// copy, which writes half of its bytes, has 6.6); with branches around the loads
+// 63, without their evict-first hint 49, without the stores' 43.8 (16384 x 4096
+// fp16: 185 instead of 177), with six CTAs an SM 46, with eight rows in flight 46.
 template <typename T>
 __global__ void __launch_bounds__(256, 5) unpermute_kernel(const T* __restrict__ x,
                                                            const float* __restrict__ w,
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(256, 5) unpermute_kernel(const T* __restrict__
     T* ov = reinterpret_cast<T*>(&o);
 #pragma unroll
     for (int e = 0; e < EPV; ++e) ov[e] = Num<T>::from_f(acc[e]);
-    reinterpret_cast<uint4*>(out)[t * vecs_per_row + v] = o;
+    __stcs(reinterpret_cast<uint4*>(out) + t * vecs_per_row + v, o);
   }
   // indices that count and leave the rows are reported
   const int64_t local = eft ? eft[n_local] : INT64_MAX;
