@@ -452,21 +452,21 @@ __global__ void expand_rows(const uint4* __restrict__ in, uint4* __restrict__ ou
 }
 
 // out[t] = dtype(sum_j fma(w[t,j], x[inv[t,j]], acc)), fp32 accumulation in
-// j order (finalizeMoeRoutingKernel, .inl:132-188).  One token per CTA, four of
-// its rows in flight by predicated loads; rows that do not count are not read.
-// Bound by memory: 8192 x 2048 bf16, top 8 (302 MB) takes 41.7 us, 7.3 TB/s (a
-// copy, which writes half of its bytes, has 6.6); with branches around the loads
-// 63, without their evict-first hint 49, without the stores' 43.8 (16384 x 4096
-// fp16: 185 instead of 177), with six CTAs an SM 46, with eight rows in flight 46.
-template <typename T>
-__global__ void __launch_bounds__(256, 5) unpermute_kernel(const T* __restrict__ x,
-                                                           const float* __restrict__ w,
-                                                           const int32_t* __restrict__ inv,
-                                                           const int64_t* eft, int n_local,
-                                                           int topk, int vecs_per_row,
-                                                           int64_t rows, T* __restrict__ out) {
+// j order (finalizeMoeRoutingKernel, .inl:132-188).  One token per CTA, G of its
+// rows in flight by predicated loads; rows that do not count are not read.
+// Bound by memory: 8192 x 2048 bf16, top 8 (302 MB) takes 49 us right after the
+// kernel that wrote x, 55 with other data in L2, 41.7 replayed over three x;
+// without the evict-first hint on the loads 57, 61 and 49, with branches around
+// them 63 replayed.  The hint on the stores is for outputs above L2's size (16384
+// x 4096 fp16 177 instead of 185 us, replayed).  Four rows and five CTAs an SM; up
+// to two experts a token two and eight: 16384 x 2048, top 1, 37 instead of 49 us
+// with other data in L2; with eight experts 48 instead of 42 replayed.
+template <typename T, int G>
+__global__ void __launch_bounds__(256, G > 2 ? 5 : 8)
+    unpermute_kernel(const T* __restrict__ x, const float* __restrict__ w,
+                     const int32_t* __restrict__ inv, const int64_t* eft, int n_local, int topk,
+                     int vecs_per_row, int64_t rows, T* __restrict__ out) {
   constexpr int EPV = 16 / sizeof(T);
-  constexpr int G = 4;  // source rows in flight
   const int64_t t = blockIdx.x;
   const int64_t valid = eft ? min(rows, static_cast<int64_t>(eft[n_local])) : rows;
   for (int v = threadIdx.x; v < vecs_per_row; v += blockDim.x) {
@@ -510,6 +510,17 @@ __global__ void __launch_bounds__(256, 5) unpermute_kernel(const T* __restrict__
       const int i = __ldg(inv + t * topk + j);
       if (i >= rows && i < local) atomicOr(&g_err_route, kErrBadIndex);
     }
+}
+
+template <typename T>
+int launch_unpermute(const void* x, int64_t rows, const float* w, const int32_t* inv,
+                     const int64_t* eft, int n_local, int n_token, int topk, int vpr, void* out,
+                     cudaStream_t st) {
+  const int threads = std::min(256, std::max(32, ((vpr + 31) / 32) * 32));
+  auto kernel = topk > 2 ? unpermute_kernel<T, 4> : unpermute_kernel<T, 2>;
+  kernel<<<n_token, threads, 0, st>>>(static_cast<const T*>(x), w, inv, eft, n_local, topk, vpr,
+                                      rows, static_cast<T*>(out));
+  return check_launch("moe_unpermute");
 }
 
 template <typename T>
@@ -874,24 +885,13 @@ int i8moe_moe_unpermute_rows(const void* permuted_hidden, int64_t n_rows, int dt
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (permuted_hidden == nullptr) n_rows = 0;
   const int vpr = static_cast<int>(row_bytes / 16);
-  const int threads = std::min(256, std::max(32, ((vpr + 31) / 32) * 32));
-  const int nl = static_cast<int>(n_local_expert);
-  const int k = static_cast<int>(topk);
-  const dim3 grid(static_cast<unsigned>(n_token));
-  if (dtype == I8MOE_BF16) {
-    unpermute_kernel<__nv_bfloat16><<<grid, threads, 0, st>>>(
-        static_cast<const __nv_bfloat16*>(permuted_hidden), topk_weights, inv_permuted_idx,
-        expert_first_token_offset, nl, k, vpr, n_rows, static_cast<__nv_bfloat16*>(out));
-  } else if (dtype == I8MOE_FP16) {
-    unpermute_kernel<__half><<<grid, threads, 0, st>>>(
-        static_cast<const __half*>(permuted_hidden), topk_weights, inv_permuted_idx,
-        expert_first_token_offset, nl, k, vpr, n_rows, static_cast<__half*>(out));
-  } else {
-    unpermute_kernel<float><<<grid, threads, 0, st>>>(
-        static_cast<const float*>(permuted_hidden), topk_weights, inv_permuted_idx,
-        expert_first_token_offset, nl, k, vpr, n_rows, static_cast<float*>(out));
-  }
-  return check_launch("moe_unpermute");
+  const int nl = static_cast<int>(n_local_expert), k = static_cast<int>(topk);
+  const int t = static_cast<int>(n_token);
+  auto launch = dtype == I8MOE_BF16   ? launch_unpermute<__nv_bfloat16>
+                : dtype == I8MOE_FP16 ? launch_unpermute<__half>
+                                      : launch_unpermute<float>;
+  return launch(permuted_hidden, n_rows, topk_weights, inv_permuted_idx, expert_first_token_offset,
+                nl, t, k, vpr, out, st);
 }
 
 int i8moe_moe_unpermute(const void* permuted_hidden, int dtype, const float* topk_weights,

@@ -90,8 +90,9 @@ __global__ void __launch_bounds__(256) scatter_rows_kernel(RowArgs a, const uint
 
 // One token per CTA, four of its rows in flight by predicated loads; rows that do
 // not count are not read.  Bound by memory: 8192 x 2048 bf16, top 8 (302 MB) takes
-// 45 us, 6.7 TB/s (a copy has 6.6), 16384 x 4096 fp16 175; without the loads'
-// evict-first hint 48, without the stores' 43 and 184.
+// 47 us right after the kernel that wrote the rows, 55 with other data in L2, 45
+// replayed over three inputs, and 16384 x 4096 fp16 175; replayed without the
+// loads' evict-first hint 48, without the stores' 43 and 184.
 template <typename T>
 __global__ void __launch_bounds__(256, 6) gather_sum_kernel(RowArgs a,
                                                             const uint4* __restrict__ rows,
