@@ -213,9 +213,12 @@ int i8moe_moe_unpermute_backward(const void* out_grad, const void* permuted_hidd
  *   y = h / sqrt(mean(h^2) + eps) * weight
  *   q_scale = max(max|y|, 1e-10) / 127,  q = rint(y / q_scale)
  * in fp32 from the unrounded h and y; residual_out (with residual only), y
- * and q are rounded once.  y, rstd (fp32 [n_rows], for the backward pass) and
- * q / q_scale may be NULL, not both y and q.  A row whose norm is not finite
- * gets q_scale NaN and q 0.  weight has the rows' dtype or I8MOE_FP32. */
+ * and q are rounded once (q's quotient is off by a few of its last bits, so
+ * that one next to a half may round to either side).  y, rstd (fp32 [n_rows],
+ * for the backward pass) and q / q_scale may be NULL, not both y and q.  A row
+ * whose norm is not finite gets q_scale NaN and q 0, and so does one whose sum
+ * of squares leaves fp32, of which y is 0.  weight has the rows' dtype or
+ * I8MOE_FP32. */
 int i8moe_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                    int dtype, const void* weight, int weight_dtype, int64_t n_rows,
                    int64_t n_hidden, float eps, void* residual_out, void* y, float* rstd,

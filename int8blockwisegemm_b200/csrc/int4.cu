@@ -182,14 +182,14 @@ struct alignas(sizeof(T) * kCount) ScalePack {
   T v[kCount];
 };
 
-// One CTA an SM: 12 warps of 160 registers take 62 us for the decode case's
-// first product, 16 of 128 (with spills) 70, 8 of 172 72.
+// One CTA an SM: 12 warps of 160 registers take 65 us for the decode case's
+// first product, 14 of 128 70 and 13 of 128 74.
 constexpr int kMvThreads = 384;
 constexpr int kMvWarps = kMvThreads / 32;
-constexpr int kMvChunk = 8;          // rows of a chunk, one n8 tile: two take 103 us in that case,
-                                     // and 49 instead of 43 with 16 rows an expert
+constexpr int kMvChunk = 8;          // rows of a chunk, one n8 tile: two took 103 us in that case
+                                     // (62 then), and 49 instead of 43 with 16 rows an expert
 constexpr int kMvStep = 128;         // columns of a step
-constexpr int kMvSlots = 2;          // steps of weights in flight: three take 64 us
+constexpr int kMvSlots = 2;          // steps of weights in flight: three take 66 us
 constexpr int kMvTileBytes = 16 * kMvStep / 2;
 constexpr int kMvMaxExperts = 2048;
 
@@ -201,9 +201,10 @@ constexpr int kMvMaxExperts = 2048;
 // sums of those that it shares with the next warps meet in shared memory, once,
 // at the end.
 //
-// Bound by instruction issue beside memory: 128 tokens' first product (256
-// experts, K 2048, 2 x 512 columns, 277 MB) takes 61 us, 4.5 TB/s; the loads
-// alone take 49 us, and without them 60.
+// Bound by latencies that three warps a scheduler leave open: 128 tokens' first
+// product (256 experts, K 2048, 2 x 512 columns, 274 MB) takes 65 us, 4.2 TB/s,
+// with 59 % of the issue slots busy, the ALU pipe 57 and the tensor pipe 25 %; the
+// loads alone take 49 us.
 //
 // A warp's weights (16 kTiles rows x 128 columns a step) come through its own
 // ring of slots in shared memory, steps ahead and across units, so that no

@@ -1,7 +1,7 @@
 // RMS norm with the residual's addition, an int8 output with a scale per
 // token, and the gradients.  No reference counterpart: it is the step in
-// front of the MoE layer, whose int8 output is what i8moe_int8_grouped_mm
-// takes with a_row_scale.
+// front of the MoE layer, whose int8 output, sorted by expert, is what
+// i8moe_int8_grouped_mm takes with a_row_scale.
 //
 //   h = x + residual                       (stored rounded to the row type)
 //   rstd = 1 / sqrt(mean(h^2) + eps)       (from the unrounded fp32 sum h)

@@ -6,8 +6,9 @@ Weights are kept as ``packed`` uint8 [E, N, K/2], column k in byte k // 2 (low
 half for even k) as q + 8 with q in [-8, 7], and ``scale`` [E, N,
 ceil(K / group_size)]; a weight is scale * q.  Activations are bf16 or fp16.
 The kernels read the weights of the experts that have rows once per eight
-rows, so they are for few rows per expert; with many, the INT8 grouped GEMMs
-are the faster way.
+rows, so they are for few rows per expert.  64 experts of 1024 x 2048: up to 8
+rows each take 22 us, where the INT8 grouped GEMM takes 31; from 12 on (36) the
+INT8 product is the faster one, with 64 rows 34 against 117 us.
 """
 
 from __future__ import annotations

@@ -5,9 +5,10 @@ reference counterpart), differentiable, and with an int8 output.
     y = h / sqrt(mean(h^2) + eps) * weight
 
 ``rms_norm`` gives y (and h, the residual stream of the next block) in x's
-type.  ``rms_norm_quant_int8`` gives y as int8 with one scale per token, the
-``a`` / ``a_row_scale`` of ``ops.int8_grouped_mm_scaled``, and on request y as
-well, for the router.  Sums, norms and scales are fp32; y and the int8 values
+type.  ``rms_norm_quant_int8`` gives y as int8 with one scale per token, and on
+request y as well, for the router.  Sorted by expert (``q[src]``, ``scale[src]``
+with src = permuted_idx // topk) they are the ``a`` and ``a_row_scale`` of
+``ops.int8_grouped_mm_scaled``.  Sums, norms and scales are fp32; y and the int8 values
 come from the unrounded h, and so do the gradients (x and residual are kept for
 them).
 
@@ -38,8 +39,10 @@ def rms_norm(x, weight, eps: float = 1e-6, residual=None):
 def rms_norm_quant_int8(x, weight, eps: float = 1e-6, residual=None, return_norm: bool = False):
     """(q int8 [..., K], scale fp32 [...], y or None, h or None): per token
     scale = max(max|y|, 1e-10) / 127 and q = rint(y / scale); y with
-    ``return_norm``, h with a residual.  A token whose norm is not finite gets
-    scale NaN and q 0.  No gradients."""
+    ``return_norm``, h with a residual.  The quotient is fp32, off by a few of
+    its last bits, so that one next to a half may round to either side.  A token
+    whose norm is not finite (or whose squares leave fp32) gets scale NaN and q
+    0.  No gradients."""
     return TORCH_OPS.rms_norm_quant_int8(x, weight, eps, residual, return_norm)
 
 
