@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import re
 from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p
 from pathlib import Path
 
@@ -121,7 +122,8 @@ def _load_torch_ops():
         from . import _torch_ops
     except ImportError as exc:
         return _NoTorchOps(f"cannot load _torch_ops.so ({exc})")
-    running = torch.__version__.split("+")[0]
+    # the header's version is without a pre-release's suffix
+    running = re.match(r"[\d.]*\d", torch.__version__).group()
     if _torch_ops.torch_version != running:
         return _NoTorchOps(f"_torch_ops.so was built against torch {_torch_ops.torch_version}, "
                            f"this is {running}")

@@ -129,3 +129,13 @@ def test_the_binding_is_rebuilt_for_another_torch(tmp_path, monkeypatch):
     build.build_torch_ops()
     build.build_torch_ops()
     assert len(built) == 2
+
+
+def test_a_pre_release_is_the_version_of_its_headers():
+    run_python("""
+import torch
+version, torch.__version__ = torch.__version__, torch.__version__.split("+")[0] + "a0+git0"
+from int8blockwisegemm_b200 import _lib
+torch.__version__ = version
+assert hasattr(_lib.TORCH_OPS, "rms_norm")
+""")
